@@ -251,6 +251,70 @@ int tsb_scatter_backward(const void *grad_out, const int64_t *index, void *grad_
 int tsb_arg_backward(const void *grad_out, const int64_t *arg, void *grad_in,
                      int64_t B, int64_t E, int64_t K, int64_t N, int dtype, tsb_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Operators on packed batches: a router's choice of experts, tokens sorted by expert and back, and the gated linear
+ * recurrence over the rows of a CSR segment.  No counterpart upstream.  Index-valued outputs are int64.
+ *
+ * expert_topk: the k experts with the largest logits[t, :] of each of T tokens, in descending order (ties towards the
+ * smaller index; a logit of -inf is never chosen: index -1, weight 0; NaN ranks above everything).
+ *   logits               [T,E] fp32 / fp16 / bf16, 1 <= k <= E <= 1024
+ *   weight               [T,k] fp32: softmax over all E logits at the chosen ones, divided by their sum if normalize
+ *   index                [T,k]
+ * expert_topk_backward: grad_logits [T,E] from grad_weight [T,k] and the forward's outputs. */
+int tsb_expert_topk(const void *logits, float *weight, int64_t *index, int64_t T, int64_t E, int64_t k, int normalize,
+                    int dtype, tsb_stream_t stream);
+int tsb_expert_topk_backward(const void *logits, const float *weight, const int64_t *index, const float *grad_weight,
+                             void *grad_logits, int64_t T, int64_t E, int64_t k, int normalize, int dtype,
+                             tsb_stream_t stream);
+
+/* expert_sort: stable counting sort of n entries by index[i] in [0, E) (others are dropped).  n < 2^31, E <= 4096.
+ *   order                [n] entry ids expert by expert, ascending inside an expert; dropped entries come last
+ *   slot                 [n] the place of entry i in order, -1 for dropped entries
+ *   indptr               [E+1] expert e owns the places [indptr[e], indptr[e+1])
+ *   workspace            tsb_expert_sort_workspace_bytes(n, E) bytes, 256-byte aligned */
+size_t tsb_expert_sort_workspace_bytes(int64_t n, int64_t E);
+int tsb_expert_sort(const int64_t *index, int64_t *slot, int64_t *order, int64_t *indptr, int64_t n, int64_t E,
+                    void *workspace, size_t workspace_bytes, tsb_stream_t stream);
+
+/* expert_spread: many[slot[t,j], :] = few[t, :] (* weight[t,j]).  few [T,K], slot [T,k], many [T*k, K]; fp32 / fp64 /
+ * fp16 / bf16.  Rows of many from *used (device pointer: indptr[E]) on are zeroed; slots outside [0, T*k) are skipped.
+ *   weight               [T,k] in the accumulation type (fp32, fp64 for fp64 data) or NULL
+ *   rows, dot            both or neither: dot[t,j] = <few[t,:], rows[slot[t,j],:]> (accumulation type, 0 where the slot
+ *                        is skipped), the gradient of the weights; rows [T*k, K] of dtype
+ * expert_fold: few[t, :] = sum over j of many[slot[t,j], :] (* weight[t,j]), summed in the accumulation type in the
+ * order of j; skipped slots add nothing.
+ *   other, dot           both or neither: dot[t,j] = <other[t,:], many[slot[t,j],:]>; other [T,K] of dtype
+ * Deterministic (no atomics). */
+int tsb_expert_spread(const void *few, const int64_t *slot, const int64_t *used, const void *weight, const void *rows,
+                      void *many, void *dot, int64_t T, int64_t k, int64_t K, int dtype, tsb_stream_t stream);
+int tsb_expert_fold(const void *many, const int64_t *slot, const void *weight, const void *other, void *few, void *dot,
+                    int64_t T, int64_t k, int64_t K, int dtype, tsb_stream_t stream);
+
+/* scan_csr: h[e] = gate[e] * h[e-1] + src[e] along each segment [indptr[n], indptr[n+1]), h before a segment's first row
+ * = state[n] (or 0).  src, out [B,E,K]; gate [B,E,K/width], each shared by `width` neighbouring channels; state, last
+ * [B,N,K] in the accumulation type (fp32, fp64 for fp64 data) or NULL.
+ *   gate_dtype           dtype, or TSB_F32 with 16-bit data
+ *   out                  rows outside every segment become 0
+ *   last                 h at each segment's last row; state[n] (or 0) for empty segments
+ * scan_csr_backward: from grad_out [B,E,K] and grad_last [B,N,K] (either may be NULL: zero), and the forward's out:
+ *   grad_src [B,E,K] of dtype, grad_gate [B,E,K/width] of gate_dtype (or NULL), grad_state [B,N,K] (or NULL).
+ *   workspace            tsb_scan_csr_backward_workspace_bytes(...) bytes, 256-byte aligned
+ * Deterministic (no atomics).
+ * scan_step: one token for each of n states: state[i,:] = gate[i,:] * state[i,:] + src[i,:] in place, out = the new
+ * state rounded to dtype.  Consecutive states are state_stride elements apart (>= K). */
+size_t tsb_scan_csr_workspace_bytes(int64_t B, int64_t E, int64_t K, int64_t N, int64_t width, int dtype, int gate_dtype);
+int tsb_scan_csr(const void *src, const void *gate, const int64_t *indptr, const void *state, void *out, void *last,
+                 int64_t B, int64_t E, int64_t K, int64_t N, int64_t width, int64_t indptr_batch_stride, int dtype,
+                 int gate_dtype, void *workspace, size_t workspace_bytes, tsb_stream_t stream);
+size_t tsb_scan_csr_backward_workspace_bytes(int64_t B, int64_t E, int64_t K, int64_t N, int64_t width, int dtype,
+                                             int gate_dtype);
+int tsb_scan_csr_backward(const void *grad_out, const void *grad_last, const void *gate, const void *out,
+                          const int64_t *indptr, const void *state, void *grad_src, void *grad_gate, void *grad_state,
+                          int64_t B, int64_t E, int64_t K, int64_t N, int64_t width, int64_t indptr_batch_stride,
+                          int dtype, int gate_dtype, void *workspace, size_t workspace_bytes, tsb_stream_t stream);
+int tsb_scan_step(const void *src, const void *gate, void *state, void *out, int64_t n, int64_t K, int64_t width,
+                  int64_t state_stride, int dtype, int gate_dtype, tsb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

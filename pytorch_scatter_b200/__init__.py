@@ -47,6 +47,8 @@ from .segment_coo import segment_mean_coo, segment_min_coo  # noqa
 from .segment_coo import segment_max_coo, segment_coo, gather_coo  # noqa
 from .composite import scatter_std, scatter_logsumexp  # noqa
 from .composite import scatter_softmax, scatter_log_softmax  # noqa
+from .expert import expert_topk, expert_sort, expert_dispatch, expert_combine  # noqa
+from .scan import scan_csr, scan_csr_state, scan_step  # noqa
 
 __all__ = [
     'scatter_sum',
@@ -74,5 +76,12 @@ __all__ = [
     'scatter_logsumexp',
     'scatter_softmax',
     'scatter_log_softmax',
+    'expert_topk',
+    'expert_sort',
+    'expert_dispatch',
+    'expert_combine',
+    'scan_csr',
+    'scan_csr_state',
+    'scan_step',
     '__version__',
 ]

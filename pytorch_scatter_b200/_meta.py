@@ -108,3 +108,50 @@ if _lib_defined:
     @torch.library.register_fake('torch_scatter::index_is_sorted')
     def _(index):
         return False   # a property of the data: traced programs take the composed (order-independent) operators
+
+    def _acc_dtype(t):
+        return torch.float64 if t.dtype == torch.float64 else torch.float32
+
+    @torch.library.register_fake('torch_scatter::_expert_topk_fw')
+    def _(logits, k, normalize):
+        shape = list(logits.shape[:-1]) + [k]
+        return logits.new_empty(shape, dtype=torch.float32), logits.new_empty(shape, dtype=torch.long)
+
+    @torch.library.register_fake('torch_scatter::_expert_topk_bw')
+    def _(grad, logits, weight, index, normalize):
+        return torch.empty_like(logits, memory_format=torch.contiguous_format)
+
+    @torch.library.register_fake('torch_scatter::_expert_sort')
+    def _(index, num_experts):
+        return (torch.empty_like(index, memory_format=torch.contiguous_format), index.new_empty((index.numel(),)),
+                index.new_empty((num_experts + 1,)))
+
+    @torch.library.register_fake('torch_scatter::_expert_spread')
+    def _(few, slot, indptr, weight, rows):
+        many = few.new_empty([slot.numel()] + list(few.shape[slot.dim() - 1:]))
+        return many, _placeholder(few) if rows is None else few.new_empty(slot.shape, dtype=_acc_dtype(few))
+
+    @torch.library.register_fake('torch_scatter::_expert_fold')
+    def _(many, slot, weight, other):
+        few = many.new_empty(list(slot.shape[:-1]) + list(many.shape[1:]))
+        return few, _placeholder(many) if other is None else many.new_empty(slot.shape, dtype=_acc_dtype(many))
+
+    def _states(src, indptr):
+        shape = list(src.shape)
+        shape[indptr.dim() - 1] = indptr.size(-1) - 1
+        return src.new_empty(shape, dtype=_acc_dtype(src))
+
+    @torch.library.register_fake('torch_scatter::_scan_csr_fw')
+    def _(src, gate, indptr, state, want_last):
+        out = torch.empty_like(src, memory_format=torch.contiguous_format)
+        return out, _states(src, indptr) if want_last else _placeholder(src)
+
+    @torch.library.register_fake('torch_scatter::_scan_csr_bw')
+    def _(grad_out, grad_last, gate, out, indptr, state, want_gate, want_state):
+        return (torch.empty_like(out, memory_format=torch.contiguous_format),
+                torch.empty_like(gate, memory_format=torch.contiguous_format) if want_gate else _placeholder(gate),
+                _states(out, indptr) if want_state else _placeholder(out))
+
+    @torch.library.register_fake('torch_scatter::_scan_step')
+    def _(src, gate, state):
+        return torch.empty_like(src, memory_format=torch.contiguous_format)

@@ -101,6 +101,44 @@ template <typename Signature> inline c10::TypedOperatorHandle<Signature> interna
 }
 inline torch::Tensor no_tensor(const torch::Tensor &like) { return torch::empty({0}, like.options()); }
 
+// The operators on packed batches have a first derivative only.  A gradient computed under create_graph passes through
+// this node, so that differentiating it again raises instead of silently giving nothing.
+class FirstOrderOnly : public torch::autograd::Function<FirstOrderOnly> {
+public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext *, torch::autograd::Variable grad, at::TensorList) {
+    return {grad.detach()};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *, torch::autograd::variable_list) {
+    TORCH_CHECK(false, "torch_scatter: this operator has no second derivative");
+  }
+};
+inline torch::autograd::variable_list first_order(torch::autograd::variable_list grads, std::vector<torch::Tensor> from) {
+  if (!at::GradMode::is_enabled()) return grads;
+  std::vector<torch::Tensor> known;
+  for (auto &t : from)
+    if (t.defined()) known.push_back(t);
+  for (auto &g : grads)
+    if (g.defined()) g = FirstOrderOnly::apply(g, at::TensorList(known))[0];
+  return grads;
+}
+
+// accumulation type of a floating dtype: fp64 for fp64, else fp32
+inline at::ScalarType acc_dtype(const torch::Tensor &t) {
+  return t.scalar_type() == at::ScalarType::Double ? at::ScalarType::Double : at::ScalarType::Float;
+}
+inline void check_float_dtype(const torch::Tensor &t, const char *name) {
+  const auto s = t.scalar_type();
+  TORCH_CHECK(s == at::ScalarType::Float || s == at::ScalarType::Double || s == at::ScalarType::Half || s == at::ScalarType::BFloat16,
+              name, " must be a float32, float64, float16 or bfloat16 tensor, got ", s);
+}
+inline const void *opt_ptr(const std::optional<torch::Tensor> &t) { return t.has_value() ? t.value().data_ptr() : nullptr; }
+inline std::optional<torch::Tensor> opt_contiguous(const std::optional<torch::Tensor> &t) {
+  return t.has_value() ? std::optional<torch::Tensor>(t.value().contiguous()) : std::nullopt;
+}
+inline std::optional<torch::Tensor> some_if_defined(const torch::Tensor &t) {
+  return t.defined() ? std::optional<torch::Tensor>(t) : std::nullopt;
+}
+
 // ---- forward/backward drivers shared by the registry files ------------------------------------
 std::tuple<torch::Tensor, std::optional<torch::Tensor>>
 segment_csr_fw(torch::Tensor src, torch::Tensor indptr, std::optional<torch::Tensor> optional_out,
