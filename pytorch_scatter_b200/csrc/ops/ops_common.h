@@ -17,6 +17,8 @@
 
 namespace tsb_ops {
 
+// Messages hold numbers as std::to_string: an integer streamed into a message needs the locale facets of the C++ runtime
+// that this file was compiled against, which need not be the one that the process has loaded.
 // Same wording as the upstream checks (csrc/cuda/utils.cuh:5-7) so callers see familiar errors.
 #define TSB_CHECK_CUDA(x) TORCH_CHECK((x).device().is_cuda(), #x " must be CUDA tensor (this build has no CPU path)")
 #define TSB_CHECK_INPUT(x) TORCH_CHECK(x, "Input mismatch")

@@ -62,8 +62,8 @@ std::tuple<torch::Tensor, torch::Tensor> expert_topk(torch::Tensor logits, int64
   TORCH_CHECK(s == at::ScalarType::Float || s == at::ScalarType::Half || s == at::ScalarType::BFloat16,
               "expert_topk: logits must be a float32, float16 or bfloat16 tensor, got ", s);
   TORCH_CHECK(logits.dim() >= 1, "expert_topk: logits must have a last dimension of experts");
-  TORCH_CHECK(logits.size(-1) >= 1 && logits.size(-1) <= 1024, "expert_topk: 1 to 1024 experts are supported, got ", logits.size(-1));
-  TORCH_CHECK(k >= 1 && k <= logits.size(-1), "expert_topk: k must be between 1 and the number of experts (", logits.size(-1), "), got ", k);
+  TORCH_CHECK(logits.size(-1) >= 1 && logits.size(-1) <= 1024, "expert_topk: 1 to 1024 experts are supported, got ", std::to_string(logits.size(-1)));
+  TORCH_CHECK(k >= 1 && k <= logits.size(-1), "expert_topk: k must be between 1 and the number of experts (", std::to_string(logits.size(-1)), "), got ", std::to_string(k));
   auto r = ExpertTopk::apply(logits, k, normalize);
   return std::make_tuple(r[0], r[1]);
 }
@@ -88,7 +88,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> sort_impl(torch::Tensor 
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> expert_sort(torch::Tensor index, int64_t num_experts) {
   TSB_CHECK_CUDA(index);
   check_index_dtype(index, "index");
-  TORCH_CHECK(num_experts >= 1 && num_experts <= 4096, "expert_sort: 1 to 4096 experts are supported, got ", num_experts);
+  TORCH_CHECK(num_experts >= 1 && num_experts <= 4096, "expert_sort: 1 to 4096 experts are supported, got ", std::to_string(num_experts));
   static auto op = internal_op<std::tuple<torch::Tensor, torch::Tensor, torch::Tensor>(torch::Tensor, int64_t)>("torch_scatter::_expert_sort");
   return op.call(index, num_experts);
 }
@@ -204,7 +204,7 @@ torch::Tensor expert_dispatch(torch::Tensor src, torch::Tensor slot, torch::Tens
 
 torch::Tensor expert_combine(torch::Tensor rows, torch::Tensor slot, torch::Tensor indptr, std::optional<torch::Tensor> weight) {
   check_plan("expert_combine", rows, slot, indptr, weight);
-  TORCH_CHECK(rows.dim() >= 1 && rows.size(0) == slot.numel(), "expert_combine: rows must have one row for each entry of slot (", slot.numel(), ")");
+  TORCH_CHECK(rows.dim() >= 1 && rows.size(0) == slot.numel(), "expert_combine: rows must have one row for each entry of slot (", std::to_string(slot.numel()), ")");
   return ExpertRows<false>::apply(rows, slot, indptr, weight)[0];
 }
 

@@ -112,7 +112,7 @@ torch::Tensor checked_gate(const char *name, const torch::Tensor &src, const tor
   TORCH_CHECK(gate.dim() == src.dim(), name, ": gate must have as many dimensions as src");
   bool as_it_is = true, shared = false;
   for (int64_t i = 0; i < src.dim(); i++) {
-    TORCH_CHECK(gate.size(i) == src.size(i) || gate.size(i) == 1, name, ": gate does not broadcast against src at dimension ", i);
+    TORCH_CHECK(gate.size(i) == src.size(i) || gate.size(i) == 1, name, ": gate does not broadcast against src at dimension ", std::to_string(i));
     if (gate.size(i) == src.size(i)) {
       if (shared && src.size(i) != 1) as_it_is = false;
     } else {
@@ -133,7 +133,7 @@ variable_list scan(const char *name, torch::Tensor src, torch::Tensor gate, torc
   TORCH_CHECK(src.dim() >= indptr.dim(), name, ": src must have at least as many dimensions as indptr");
   const int64_t dim = indptr.dim() - 1;
   for (int64_t i = 0; i < dim; i++)
-    TORCH_CHECK(indptr.size(i) == src.size(i) || indptr.size(i) == 1, name, ": indptr does not broadcast against src at dimension ", i);
+    TORCH_CHECK(indptr.size(i) == src.size(i) || indptr.size(i) == 1, name, ": indptr does not broadcast against src at dimension ", std::to_string(i));
   gate = checked_gate(name, src, gate, dim);
   if (state.has_value()) {
     const auto &s = state.value();

@@ -30,7 +30,7 @@ def test_cpu_tensors_fail_loudly():
 
 
 def cuda(*shape, dtype=torch.float32):
-    return torch.empty(*shape, dtype=dtype, device='cuda')
+    return torch.empty(shape, dtype=dtype, device='cuda')
 
 
 def test_fake_tensor_shapes():
