@@ -31,7 +31,7 @@ int check(int64_t B, int64_t E, int64_t K, int64_t N, int64_t width, int dtype, 
   if (B < 0 || E < 0 || K < 0 || N < 0 || width < 1 || K % width != 0) return TSB_ERR_ARG;
   if (dtype != TSB_F32 && dtype != TSB_F64 && dtype != TSB_F16 && dtype != TSB_BF16) return TSB_ERR_DTYPE;
   if (gate_dtype != dtype && !(gate_dtype == TSB_F32 && dtype != TSB_F64)) return TSB_ERR_DTYPE;
-  if (N >= 2147483647LL) return TSB_ERR_TOO_LARGE;
+  if (N >= scan::kMostSegments) return TSB_ERR_TOO_LARGE;
   return TSB_OK;
 }
 

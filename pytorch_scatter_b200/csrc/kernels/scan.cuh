@@ -8,15 +8,18 @@
 //
 // Both are affine maps of the running value, value' = A * value + B, and maps compose: rows are cut into tiles of L rows,
 // and every input is read from HBM once.  A thread owns VEC channels (16 bytes) of R consecutive rows of a tile, which it
-// copies to its own slots of shared memory kStages tiles ahead (cp.async; nobody else reads them, so the data needs no
-// barrier).  (1) It composes its rows' maps; (2) the maps are scanned over the threads of a warp by shuffles, over the
-// warps through shared memory and over the CTAs of a cluster, which hold neighbouring tiles of the same channels, through
-// distributed shared memory; (3) it walks its rows again from the value that reaches them and writes the outputs.  The
-// cluster then moves on by its CTAs' tiles, carrying the value along, so that one launch covers any length without
-// waiting on anything but its own cluster.  The composition has a fixed shape: results do not vary from run to run.
+// copies to its own slots of shared memory two tiles ahead (cp.async; nobody else reads them, so the data needs no
+// barrier).  (1) It composes its rows' maps and leaves the result in shared memory.  (2) Turned over, a thread takes VEC
+// consecutive maps of one channel, composes them and scans over the lanes that share the channel; the CTAs of a cluster
+// hold neighbouring tiles of the same channels and exchange their totals through distributed shared memory; then the
+// value that reaches each thread's rows is known.  (3) Each thread walks its rows again from that value and writes the
+// outputs.  The cluster moves on by its CTAs' tiles, carrying the value along in registers, so that one launch covers any
+// length without waiting on anything but its own cluster.  The composition has a fixed shape: results do not vary from
+// run to run.
 //
 // A segment's first row (backward: its last) does not take the value from the row before: such a map is marked `reset`
-// and drops what comes in, so infinities and NaN of one segment never reach the next.
+// and drops what comes in, so infinities and NaN of one segment never reach the next.  Tiles that no segment border
+// touches run a copy of the code without these checks.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -30,7 +33,6 @@ namespace tsb {
 namespace scan {
 
 constexpr int kScanThreads = 128;
-constexpr int kScanWarps = kScanThreads / 32;
 constexpr int kStages = 3;
 constexpr int kMostCluster = 8;
 
@@ -45,33 +47,33 @@ struct ScanParams {
   int lx_log2, cluster, lanes_log2;  // lanes_log2: lanes of one row whose gate products are summed by shuffles
 };
 
-// row flags
-constexpr int kStart = 1, kEnd = 2, kDead = 4, kPad = 8;
-struct Mark { int seg, flags; };
+// row marks: the row's segment and flags
+constexpr int kStart = 1, kEnd = 2, kDead = 4, kPad = 8, kMarkBits = 4;
+constexpr int64_t kMostSegments = (int64_t)1 << 27;
 
 // A copy of VEC values to the thread's own slot.  One 2-byte value travels in the 4-byte word that holds it (cp.async has
-// no smaller form), unless that word reaches over the array's ends.
+// no smaller form), unless that word reaches over the array's ends; `half` says which half it is.
 template <typename T, int VEC> struct Slot {
   static constexpr bool kWord = sizeof(T) * VEC == 2;
   static constexpr int kBytes = kWord ? 4 : (int)sizeof(T) * VEC;
+  static __device__ __forceinline__ int half(const T *p) { return kWord ? (int)(reinterpret_cast<uintptr_t>(p) >> 1) & 1 : 0; }
   static __device__ __forceinline__ void copy(char *slot, const T *p, const T *lo, const T *hi) {
     if constexpr (kWord) {
       const uintptr_t word = reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3;
-      const bool high = reinterpret_cast<uintptr_t>(p) & 2;
       if (word >= reinterpret_cast<uintptr_t>(lo) && word + 4 <= reinterpret_cast<uintptr_t>(hi)) {
         const unsigned dst = (unsigned)__cvta_generic_to_shared(slot);
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(word) : "memory");
       } else {
-        reinterpret_cast<T *>(slot)[high] = *p;
+        reinterpret_cast<T *>(slot)[half(p)] = *p;
       }
     } else {
       async_copy_pack<T, VEC>(reinterpret_cast<Pack<T, VEC> *>(slot), p);
     }
   }
-  static __device__ __forceinline__ Pack<T, VEC> get(const char *slot, const T *p) {
+  static __device__ __forceinline__ Pack<T, VEC> get(const char *slot, int half) {
     if constexpr (kWord) {
       Pack<T, VEC> r;
-      r.v[0] = reinterpret_cast<const T *>(slot)[(reinterpret_cast<uintptr_t>(p) >> 1) & 1];
+      r.v[0] = reinterpret_cast<const T *>(slot)[half];
       return r;
     } else {
       return *reinterpret_cast<const Pack<T, VEC> *>(slot);
@@ -90,10 +92,43 @@ template <typename A, int VEC> __device__ __forceinline__ void store_acc(const A
   for (int i = 0; i < VEC; ++i) p[at + i] = v[i];
 }
 
+// VEC values of one thread to and from shared memory, 16 bytes at a time where there are as many
+template <typename A, int VEC> __device__ __forceinline__ void put(A *p, const A (&v)[VEC]) {
+  constexpr int n = VEC * sizeof(A) >= 16 ? 16 / (int)sizeof(A) : VEC;
+#pragma unroll
+  for (int i = 0; i < VEC; i += n) {
+    Pack<A, n> q;
+#pragma unroll
+    for (int j = 0; j < n; ++j) q.v[j] = v[i + j];
+    *reinterpret_cast<Pack<A, n> *>(p + i) = q;
+  }
+}
+template <typename A, int VEC> __device__ __forceinline__ void take(A (&v)[VEC], const A *p) {
+  constexpr int n = VEC * sizeof(A) >= 16 ? 16 / (int)sizeof(A) : VEC;
+#pragma unroll
+  for (int i = 0; i < VEC; i += n) {
+    const Pack<A, n> q = *reinterpret_cast<const Pack<A, n> *>(p + i);
+#pragma unroll
+    for (int j = 0; j < n; ++j) v[i + j] = q.v[j];
+  }
+}
+
+// Round to the output's type, once; pairs of 16-bit values in one instruction.
+template <typename T, int VEC, typename A> __device__ __forceinline__ void round_pack(Pack<T, VEC> &o, const A (&v)[VEC]) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value && VEC % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) *reinterpret_cast<__nv_bfloat162 *>(&o.v[i]) = __floats2bfloat162_rn(v[i], v[i + 1]);
+  } else if constexpr (std::is_same<T, __half>::value && VEC % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) *reinterpret_cast<__half2 *>(&o.v[i]) = __floats2half2_rn(v[i], v[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o.v[i] = from_acc<T>(v[i]);
+  }
+}
+
 // A * h + B.  The product of a tile's gates may overflow where the recurrence itself stays at zero.
 template <typename A> __device__ __forceinline__ A apply_map(A a, A b, A h) { return h == (A)0 ? b : a * h + b; }
-
-template <typename A> __device__ __forceinline__ A shfl_up(A v, int d) { return __shfl_up_sync(kFullMask, v, d); }
 
 // first index in [lo, hi) with indptr[index] > row (UPPER) or >= row; hi if there is none
 template <bool UPPER> __device__ __forceinline__ int64_t bound(const int64_t *indptr, int64_t lo, int64_t hi, int64_t row) {
@@ -122,24 +157,27 @@ template <typename T, typename G, int VEC, bool SHARED, bool BWD> struct ScanSha
   using SrcSlot = Slot<T, VEC>;
   using GateSlot = Slot<G, kGateVec>;
   static constexpr int kRowBytes = SrcSlot::kBytes * (BWD ? 2 : 1) + GateSlot::kBytes;
-  // rows of a thread: 256 bytes of a stage at most, so that two CTAs and more fit an SM
-  static constexpr int kRows = kRowBytes * 16 <= 256 ? 16 : kRowBytes * 8 <= 256 ? 8 : 4;
+  // rows of a thread: 28 KB for each of the three stages at most, so that two CTAs and more fit an SM
+  static constexpr int kRows = 224 / kRowBytes < 16 ? 224 / kRowBytes : 16;
   static constexpr int kStageBytes = kScanThreads * kRows * kRowBytes;
+  static constexpr int kMapBytes = 2 * kScanThreads * VEC * (int)sizeof(A);  // [A, B][ty][C]
   static size_t bytes(int lx, int cluster) {
     const size_t C = (size_t)lx * VEC, L = (size_t)(kScanThreads / lx) * kRows;
-    return (size_t)kStages * kStageBytes + sizeof(A) * C * (4 * kScanWarps + 2 + (cluster > 1 ? 4 * cluster : 0)) +
-           sizeof(Mark) * 2 * L;
+    return (size_t)kStages * kStageBytes + kMapBytes + (cluster > 1 ? sizeof(A) * C * 4 * cluster : 0) + sizeof(int) * 2 * L;
   }
 };
 
 template <typename T, typename G, int VEC, bool SHARED, bool BWD>
 __global__ void __launch_bounds__(kScanThreads) scan_kernel(ScanParams p) {
   using S = ScanShape<T, G, VEC, SHARED, BWD>;
+  using SrcSlot = typename S::SrcSlot;
+  using GateSlot = typename S::GateSlot;
   using A = acc_t<T>;
   constexpr int R = S::kRows;
+  constexpr int kSrcRow = kScanThreads * SrcSlot::kBytes, kGateRow = kScanThreads * GateSlot::kBytes;
   namespace cg = cooperative_groups;
 
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x;
   const int lx = 1 << p.lx_log2, C = lx * VEC, L = (kScanThreads >> p.lx_log2) * R;
   const int col = tid & (lx - 1), ty = tid >> p.lx_log2;
   const int cs = p.cluster, rank = (int)(blockIdx.x % cs);
@@ -152,84 +190,289 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(ScanParams p) {
   const int64_t lo = part_begin(p, indptr, part), hi = part_begin(p, indptr, part + 1);
   const int64_t len = hi - lo;
   if (len <= 0) return;  // the same for the whole cluster
-  const int64_t rounds = (len + (int64_t)cs * L - 1) / ((int64_t)cs * L);
+  const int64_t step = (int64_t)cs * L;
 
   const int64_t c0 = kt * C + (int64_t)col * VEC;   // this thread's first channel
   const bool live = c0 < p.K;
   const int64_t gates = p.K / p.width, g0 = SHARED ? c0 / p.width : c0;
+  // this thread's pointers to row 0, and the way to its next row
   const T *src = static_cast<const T *>(p.src) + (p.src ? b * p.E * p.K + c0 : 0);
-  const T *fwd = static_cast<const T *>(p.fwd) + (BWD ? b * p.E * p.K + c0 : 0);
+  const T *fwd = static_cast<const T *>(p.fwd) + (BWD ? (b * p.E - 1) * p.K + c0 : 0);  // h of the row before
   const G *gate = static_cast<const G *>(p.gate) + b * p.E * gates + g0;
   T *out = static_cast<T *>(p.out) + b * p.E * p.K + c0;
+  const int64_t dk = BWD ? -p.K : p.K, dgates = BWD ? -gates : gates;
   const int64_t srow = b * p.N;                     // first row of this batch in the state arrays
-
-  extern __shared__ __align__(128) char smem[];
-  char *s_src = smem;                                              // [stage][row][thread]
-  char *s_fwd = s_src + kStages * R * kScanThreads * S::SrcSlot::kBytes;
-  char *s_gate = s_fwd + (BWD ? kStages * R * kScanThreads * S::SrcSlot::kBytes : 0);
-  A *s_maps = reinterpret_cast<A *>(smem + (size_t)kStages * S::kStageBytes);  // maps of the warps [2][A, B][warp][C]
-  A *s_in = s_maps + 4 * kScanWarps * C;                                 // value that reaches this CTA's tile [C]
-  A *s_carry = s_in + C;                                           // value that reaches the cluster's tiles [C]
-  A *s_ca = s_carry + C;                                           // maps of the cluster's CTAs [2][cs][C]
-  A *s_cb = s_ca + (cs > 1 ? 2 * cs * C : 0);
-  Mark *s_mark = reinterpret_cast<Mark *>(s_cb + (cs > 1 ? 2 * cs * C : 0));  // [2][L]
-  __shared__ int s_resets[2][kScanWarps], s_creset[2][kMostCluster];
-  __shared__ int64_t s_found[2][2];                                // [parity]: bound of the tile's last row, next border
-
-  for (int c = tid; c < C; c += kScanThreads) s_carry[c] = 0;
-  if (cs > 1) cg::this_cluster().sync();  // all CTAs run before anyone writes to their shared memory
-
-  const auto row_of = [&](int64_t pos) { return BWD ? hi - 1 - pos : lo + pos; };
-  const auto slot = [&](char *base, int bytes, int stage, int r) { return base + (size_t)((stage * R + r) * kScanThreads + tid) * bytes; };
-  const auto first_pos = [&](int64_t i) { return (i * cs + rank) * (int64_t)L; };
-
+  const bool have_src = !BWD || p.src, want_gate = BWD && p.grad_gate;
   const T *src_lo = static_cast<const T *>(p.src), *src_hi = src_lo + p.B * p.E * p.K;
   const T *fwd_lo = static_cast<const T *>(p.fwd), *fwd_hi = fwd_lo + p.B * p.E * p.K;
   const G *gate_lo = static_cast<const G *>(p.gate), *gate_hi = gate_lo + p.B * p.E * gates;
 
-  const auto load_tile = [&](int64_t i) {
-    if (i < rounds && live) {
-      const int64_t pos = first_pos(i) + (int64_t)ty * R;
-      const int stage = (int)(i % kStages);
+  extern __shared__ __align__(128) char smem[];
+  char *s_src = smem + tid * SrcSlot::kBytes;                      // [stage][row][thread], from here on this thread's
+  char *s_fwd = s_src + kStages * R * kSrcRow;
+  char *s_gate = smem + kStages * R * kSrcRow * (BWD ? 2 : 1) + tid * GateSlot::kBytes;
+  A *s_a = reinterpret_cast<A *>(smem + (size_t)kStages * S::kStageBytes);  // maps of the threads [ty][C]; then the values
+  A *s_b = s_a + kScanThreads * VEC;                               // that reach them, in place of A
+  A *s_total = s_b + kScanThreads * VEC;                           // maps of the cluster's CTAs [2][cs][C][A, B]
+  int *s_marks = reinterpret_cast<int *>(s_total + (cs > 1 ? 4 * cs * C : 0));  // [2][L]
+  __shared__ int s_reset[kScanThreads], s_total_reset[2][kMostCluster];
+  __shared__ int64_t s_found[2][2];                                // bound of the tile's last row, next border
+
+  if (cs > 1) cg::this_cluster().sync();  // all CTAs run before anyone writes to their shared memory
+
+  const auto row_of = [&](int64_t pos) { return BWD ? hi - 1 - pos : lo + pos; };
+
+  const auto load_tile = [&](int64_t tile, int stage) {
+    const int64_t pos = tile + ty * R;
+    if (live && pos < len) {
+      const int n = (int)(len - pos < R ? len - pos : R);
+      const int64_t t = row_of(pos);
+      const T *xs = src + t * p.K, *fs = fwd + t * p.K;
+      const G *gs = gate + t * gates;
+      char *xd = s_src + stage * (R * kSrcRow), *fd = s_fwd + stage * (R * kSrcRow), *gd = s_gate + stage * (R * kGateRow);
+      const auto rows = [&](auto whole) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        if (pos + r >= len) break;
-        const int64_t t = row_of(pos + r);
-        if (!BWD || p.src) S::SrcSlot::copy(slot(s_src, S::SrcSlot::kBytes, stage, r), src + t * p.K, src_lo, src_hi);
-        S::GateSlot::copy(slot(s_gate, S::GateSlot::kBytes, stage, r), gate + t * gates, gate_lo, gate_hi);
-        if (BWD && p.grad_gate && t > 0) S::SrcSlot::copy(slot(s_fwd, S::SrcSlot::kBytes, stage, r), fwd + (t - 1) * p.K, fwd_lo, fwd_hi);
-      }
+        for (int r = 0; r < R; ++r) {
+          if (!decltype(whole)::value && r >= n) break;
+          if (have_src) SrcSlot::copy(xd + r * kSrcRow, xs, src_lo, src_hi);
+          GateSlot::copy(gd + r * kGateRow, gs, gate_lo, gate_hi);
+          if (want_gate && fs >= fwd_lo) SrcSlot::copy(fd + r * kSrcRow, fs, fwd_lo, fwd_hi);  // (row 0 has none before it)
+          xs += dk;
+          fs += dk;
+          gs += dgates;
+        }
+      };
+      if (n == R) rows(std::true_type());
+      else rows(std::false_type());
     }
     async_commit();
   };
 
-  for (int i = 0; i < kStages - 1; ++i) load_tile(i);
-
-  // the row that was looked up last: its bound, the next border on the way (none: never met), whether it is outside
+  // the row that was looked up last: its bound, the next border on the way, whether it is outside
   int64_t cursor = BWD ? p.N + 1 : 0, border = BWD ? (int64_t)1 << 62 : -1;
   bool outside = false;
+  // (2) runs with the roles turned over: channel fc, the fh-th of H lanes that share it
+  const int hbits = 31 - __clz(kScanThreads) - p.lx_log2 - (31 - __clz(VEC)), H = 1 << hbits;
+  const int fc = tid >> hbits, fh = tid & (H - 1);
+  A carry = 0;  // the value that reaches the cluster's tiles in channel fc
 
-  for (int64_t i = 0; i < rounds; ++i) {
-    load_tile(i + kStages - 1);
-    const int par = (int)(i & 1), stage = (int)(i % kStages);
-    const int64_t tile = first_pos(i);
-    // borders touch this tile: a boundary at its rows or right behind its last one
+  const auto tile_work = [&](auto has_marks, int64_t tile, int stage, int par) {
+    constexpr bool MARKED = decltype(has_marks)::value;
+    const int *mark = s_marks + par * L + ty * R;
+    const int64_t t0 = row_of(tile + ty * R);
+    const char *xs = s_src + stage * (R * kSrcRow), *fs = s_fwd + stage * (R * kSrcRow), *gs = s_gate + stage * (R * kGateRow);
+    // which half of its word the r-th row's value is in (2-byte slots only)
+    const int xhalf = SrcSlot::half(src + t0 * p.K), fhalf = SrcSlot::half(fwd + t0 * p.K), ghalf = GateSlot::half(gate + t0 * gates);
+    const int kodd = (int)(p.K & 1), godd = (int)(gates & 1);
+
+    // ---- (1) the map of this thread's rows
+    {
+      A ma[VEC], mb[VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) { ma[v] = 1; mb[v] = 0; }
+      int reset = 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if constexpr (MARKED) {
+          const int m = mark[r];
+          if (m & kPad) continue;
+          if (m & (kDead | (BWD ? kEnd : kStart))) {
+            reset = 1;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) mb[v] = 0;
+            if (m & kDead) continue;
+            if (live) load_acc<A, VEC>(mb, p.state, (srow + (m >> kMarkBits)) * p.K + c0);
+          }
+        }
+        const Pack<T, VEC> x = SrcSlot::get(xs + r * kSrcRow, (xhalf + r * kodd) & 1);
+        const Pack<G, S::kGateVec> g = GateSlot::get(gs + r * kGateRow, (ghalf + r * godd) & 1);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          const A gv = to_acc<G>(g.v[SHARED ? 0 : v]);
+          if constexpr (BWD) mb[v] = gv * (have_src ? mb[v] + to_acc<T>(x.v[v]) : mb[v]);
+          else mb[v] = gv * mb[v] + to_acc<T>(x.v[v]);
+          if (!SHARED || v == 0) ma[v] *= gv;
+        }
+      }
+      A *pa = s_a + tid * VEC, *pb = s_b + tid * VEC;
+      if constexpr (SHARED) {
+#pragma unroll
+        for (int v = 1; v < VEC; ++v) ma[v] = ma[0];
+      }
+      put(pa, ma);
+      put(pb, mb);
+      if (MARKED && col == 0) s_reset[ty] = reset;
+    }
+    __syncthreads();
+
+    // ---- (2) scan of the maps over the tile and the cluster
+    A fa[VEC], fb[VEC];
+    unsigned fr = 0;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const int at = (fh * VEC + j) * C + fc;
+      fa[j] = s_a[at];
+      fb[j] = s_b[at];
+      if (MARKED) fr |= (unsigned)s_reset[fh * VEC + j] << j;
+    }
+    A ta = fa[0], tb = fb[0];
+    int tr = fr & 1;
+#pragma unroll
+    for (int j = 1; j < VEC; ++j) {
+      const bool rs = MARKED && (fr >> j & 1);
+      tb = rs ? fb[j] : apply_map(fa[j], fb[j], tb);
+      ta *= fa[j];
+      tr |= rs;
+    }
+    for (int d = 1; d < H; d <<= 1) {
+      const A pa = __shfl_up_sync(kFullMask, ta, d, H), pb = __shfl_up_sync(kFullMask, tb, d, H);
+      const int pr = MARKED ? __shfl_up_sync(kFullMask, tr, d, H) : 0;
+      if (fh >= d) {
+        if (!MARKED || !tr) tb = apply_map(ta, tb, pb);
+        ta *= pa;
+        tr |= pr;
+      }
+    }
+    // map of the lanes before this one
+    const A ea = __shfl_up_sync(kFullMask, ta, 1, H), eb = __shfl_up_sync(kFullMask, tb, 1, H);
+    const int er = MARKED ? __shfl_up_sync(kFullMask, tr, 1, H) : 0;
+    // map of the whole tile
+    const A wa = __shfl_sync(kFullMask, ta, H - 1, H), wb = __shfl_sync(kFullMask, tb, H - 1, H);
+    const int wr = MARKED ? __shfl_sync(kFullMask, tr, H - 1, H) : 0;
+    A h = carry;
+    if (cs > 1) {
+      cg::cluster_group cluster = cg::this_cluster();
+      A *mine = s_total + ((size_t)(par * cs + rank) * C + fc) * 2;
+      for (int q = fh; q < cs; q += H) {
+        A *there = cluster.map_shared_rank(mine, q);
+        there[0] = wa;
+        there[1] = wb;
+      }
+      if (tid < cs) *cluster.map_shared_rank(&s_total_reset[par][rank], tid) = wr;
+      cluster.sync();
+      A all = carry;
+      for (int q = 0; q < cs; ++q) {
+        if (q == rank) h = all;
+        const A *m = s_total + ((size_t)(par * cs + q) * C + fc) * 2;
+        const A a = m[0], bb = m[1];
+        all = s_total_reset[par][q] ? bb : apply_map(a, bb, all);
+      }
+      carry = all;
+    } else {
+      carry = wr ? wb : apply_map(wa, wb, carry);
+    }
+    if (fh > 0) h = er ? eb : apply_map(ea, eb, h);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      s_a[(fh * VEC + j) * C + fc] = h;
+      h = MARKED && (fr >> j & 1) ? fb[j] : apply_map(fa[j], fb[j], h);
+    }
+    __syncthreads();
+
+    // ---- (3) the rows, from the value that reaches them
+    A v_[VEC];
+    take(v_, s_a + tid * VEC);
+    T *os = out + t0 * p.K;
+    int64_t t = t0;
+#pragma unroll
+    for (int r = 0; r < R; ++r, os += dk, t += BWD ? -1 : 1) {
+      int m = 0;
+      if constexpr (MARKED) {
+        m = mark[r];
+        if (m & kPad) continue;
+        if (m & (BWD ? kEnd : kStart)) {
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) v_[v] = 0;
+          if (live) load_acc<A, VEC>(v_, p.state, (srow + (m >> kMarkBits)) * p.K + c0);
+        }
+      }
+      const bool dead = MARKED && (m & kDead);
+      const Pack<T, VEC> x = SrcSlot::get(xs + r * kSrcRow, (xhalf + r * kodd) & 1);
+      const Pack<G, S::kGateVec> g = GateSlot::get(gs + r * kGateRow, (ghalf + r * godd) & 1);
+      Pack<T, VEC> o;
+      if constexpr (!BWD) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          v_[v] = to_acc<G>(g.v[SHARED ? 0 : v]) * v_[v] + to_acc<T>(x.v[v]);
+          if (dead) v_[v] = 0;
+        }
+        round_pack(o, v_);
+        if (live) {
+          st_stream<T, VEC>(os, o);
+          if (MARKED && (m & kEnd) && p.last) store_acc<A, VEC>(v_, p.last, (srow + (m >> kMarkBits)) * p.K + c0);
+        }
+      } else {
+        A dh[VEC], dg[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          dh[v] = have_src ? v_[v] + to_acc<T>(x.v[v]) : v_[v];
+          if (dead) dh[v] = 0;
+        }
+        round_pack(o, dh);
+        if (live) st_stream<T, VEC>(os, o);
+        if (want_gate) {
+          const Pack<T, VEC> f = SrcSlot::get(fs + r * kSrcRow, (fhalf + r * kodd) & 1);
+          if (MARKED && (m & kStart)) {
+            A before[VEC];
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) before[v] = 0;
+            if (live) load_acc<A, VEC>(before, p.init, (srow + (m >> kMarkBits)) * p.K + c0);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) dg[v] = dh[v] * before[v];
+          } else {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) dg[v] = dead ? (A)0 : dh[v] * to_acc<T>(f.v[v]);
+          }
+          if constexpr (!SHARED) {
+            Pack<G, VEC> og;
+            round_pack(og, dg);
+            if (live) st_stream<G, VEC>(static_cast<G *>(p.grad_gate) + (b * p.E + t) * gates + c0, og);
+          } else {
+            // sum of the thread's channels, then of the neighbouring lanes that hold the same gate; the lanes of a row
+            // are here together: rows are skipped (kPad) by whole rows
+            A sum = dg[0];
+#pragma unroll
+            for (int v = 1; v < VEC; ++v) sum += dg[v];
+            const unsigned rowmask = lx == 32 ? kFullMask : ((1u << lx) - 1u) << ((tid & 31) & ~(lx - 1));
+            for (int d = 1; d < (1 << p.lanes_log2); d <<= 1) sum += __shfl_xor_sync(rowmask, sum, d);
+            if (live && (col & ((1 << p.lanes_log2) - 1)) == 0) {
+              const int64_t per = VEC << p.lanes_log2;
+              if (per == p.width) static_cast<G *>(p.grad_gate)[(b * p.E + t) * gates + g0] = from_acc<G>(sum);
+              else static_cast<A *>(p.partial)[(b * p.E + t) * (p.K / per) + c0 / per] = sum;
+            }
+          }
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) v_[v] = dead ? (A)0 : to_acc<G>(g.v[SHARED ? 0 : v]) * dh[v];
+        if (MARKED && live && (m & kStart) && p.last) store_acc<A, VEC>(v_, p.last, (srow + (m >> kMarkBits)) * p.K + c0);
+      }
+    }
+  };
+
+  int64_t tile = (int64_t)rank * L, ahead = tile;
+  int stage = 0, ahead_stage = 0, par = 0;
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    load_tile(ahead, ahead_stage);
+    ahead += step;
+    ++ahead_stage;
+  }
+  for (int64_t done = 0; done < len; done += step) {
+    load_tile(ahead, ahead_stage);
+    ahead += step;
+    ahead_stage = ahead_stage == kStages - 1 ? 0 : ahead_stage + 1;
+    // does a border touch this tile: at one of its rows, or right behind its last one?
     const int64_t edge = BWD ? row_of(tile + L - 1) : row_of(tile) + L;
     const bool marked = outside || tile + L > len || (BWD ? border >= edge : border <= edge);
-    // what the slowest warp may still read of the tile before is kept: these alternate
-    Mark *mark = s_mark + par * L;
-    A *s_wa = s_maps + par * 2 * kScanWarps * C, *s_wb = s_wa + kScanWarps * C;
-    int *s_wreset = s_resets[par];
     if (marked) {
       for (int j = tid; j < L; j += kScanThreads) {
-        const int64_t pos = tile + j < len ? tile + j : len - 1;
-        const int64_t t = row_of(pos);
+        const int64_t t = row_of(tile + j < len ? tile + j : len - 1);
         const int64_t u = BWD ? bound<true>(indptr, 0, cursor, t) : bound<true>(indptr, cursor, p.N + 1, t);
-        Mark m{(int)(u - 1), 0};
-        if (tile + j >= len) m.flags = kPad;
-        else if (u < 1 || u > p.N) m.flags = kDead;
-        else m.flags = (indptr[u - 1] == t ? kStart : 0) | (indptr[u] == t + 1 ? kEnd : 0);
-        mark[j] = m;
+        int flags;
+        if (tile + j >= len) flags = kPad;
+        else if (u < 1 || u > p.N) flags = kDead;
+        else flags = (int)(u - 1) << kMarkBits | (indptr[u - 1] == t ? kStart : 0) | (indptr[u] == t + 1 ? kEnd : 0);
+        s_marks[par * L + j] = flags;
         if (j == L - 1) {
           s_found[par][0] = u;
           s_found[par][1] = BWD ? (u > 0 ? indptr[u - 1] : -1) : (u <= p.N ? indptr[u] : (int64_t)1 << 62);
@@ -242,214 +485,13 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(ScanParams p) {
       cursor = s_found[par][0];
       border = s_found[par][1];
       outside = cursor < 1 || cursor > p.N;
-    }
-
-    // ---- (1) the map of this thread's rows
-    A ma[VEC], mb[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) { ma[v] = 1; mb[v] = 0; }
-    int reset = 0;
-    const int64_t pos0 = tile + (int64_t)ty * R;
-    const auto get_src = [&](int r, int64_t t) { return S::SrcSlot::get(slot(s_src, S::SrcSlot::kBytes, stage, r), src + t * p.K); };
-    const auto get_gate = [&](int r, int64_t t) { return S::GateSlot::get(slot(s_gate, S::GateSlot::kBytes, stage, r), gate + t * gates); };
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int64_t t = row_of(pos0 + r);
-      if (marked) {
-        const Mark m = mark[ty * R + r];
-        if (m.flags & kPad) continue;
-        if (m.flags & kDead) {
-          reset = 1;
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) mb[v] = 0;
-          continue;
-        }
-        if (m.flags & (BWD ? kEnd : kStart)) {
-          reset = 1;
-          if (live) load_acc<A, VEC>(mb, p.state, (srow + m.seg) * p.K + c0);
-        }
-      }
-      const Pack<T, VEC> x = get_src(r, t);
-      const Pack<G, S::kGateVec> g = get_gate(r, t);
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const A gv = to_acc<G>(g.v[SHARED ? 0 : v]);
-        const A xv = !BWD || p.src ? to_acc<T>(x.v[v]) : (A)0;
-        mb[v] = BWD ? gv * (mb[v] + xv) : gv * mb[v] + xv;
-        ma[v] *= gv;
-      }
-    }
-
-    // ---- (2) scan of the maps over the warp, then over the warps and the cluster
-    A ea[VEC], eb[VEC];  // map of the lanes before this one
-    int ereset;
-    {
-      int ir = reset;
-      for (int d = lx; d < 32; d <<= 1) {
-        const int pr = __shfl_up_sync(kFullMask, ir, d);
-        const bool take = lane >= d;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const A pa = shfl_up(ma[v], d), pb = shfl_up(mb[v], d);
-          if (take && !ir) {
-            mb[v] = apply_map(ma[v], mb[v], pb);
-            ma[v] *= pa;
-          }
-        }
-        if (take) ir |= pr;
-      }
-      reset = ir;
-      ereset = __shfl_up_sync(kFullMask, ir, lx);
-      const bool head = lane < lx || lx == 32;
-      if (head) ereset = 0;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        ea[v] = shfl_up(ma[v], lx);
-        eb[v] = shfl_up(mb[v], lx);
-        if (head) { ea[v] = 1; eb[v] = 0; }
-      }
-    }
-    if (lane >= 32 - lx) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        s_wa[warp * C + col * VEC + v] = ma[v];
-        s_wb[warp * C + col * VEC + v] = mb[v];
-      }
-      if (lane == 31) s_wreset[warp] = reset;
-    }
-    __syncthreads();
-
-    if (cs > 1) {
-      cg::cluster_group cluster = cg::this_cluster();
-      int any = 0;
-#pragma unroll
-      for (int w = 0; w < kScanWarps; ++w) any |= s_wreset[w];
-      for (int c = tid; c < C; c += kScanThreads) {
-        A a = 1, bb = 0;
-#pragma unroll
-        for (int w = 0; w < kScanWarps; ++w) {
-          const A wa = s_wa[w * C + c], wb = s_wb[w * C + c];
-          bb = s_wreset[w] ? wb : apply_map(wa, wb, bb);
-          a *= wa;
-        }
-        for (int q = 0; q < cs; ++q) {
-          cluster.map_shared_rank(s_ca, q)[(par * cs + rank) * C + c] = a;
-          cluster.map_shared_rank(s_cb, q)[(par * cs + rank) * C + c] = bb;
-        }
-      }
-      if (tid < cs) cluster.map_shared_rank(&s_creset[0][0], tid)[par * kMostCluster + rank] = any;
-      cluster.sync();
-      for (int c = tid; c < C; c += kScanThreads) {
-        A h = s_carry[c];
-        for (int q = 0; q < cs; ++q) {
-          if (q == rank) s_in[c] = h;
-          const A a = s_ca[(par * cs + q) * C + c], bb = s_cb[(par * cs + q) * C + c];
-          h = s_creset[par][q] ? bb : apply_map(a, bb, h);
-        }
-        s_carry[c] = h;
-      }
+      tile_work(std::true_type(), tile, stage, par);
     } else {
-      for (int c = tid; c < C; c += kScanThreads) {
-        A h = s_carry[c];
-        s_in[c] = h;
-#pragma unroll
-        for (int w = 0; w < kScanWarps; ++w) {
-          const A a = s_wa[w * C + c], bb = s_wb[w * C + c];
-          h = s_wreset[w] ? bb : apply_map(a, bb, h);
-        }
-        s_carry[c] = h;
-      }
+      tile_work(std::false_type(), tile, stage, par);
     }
-    __syncthreads();
-
-    // ---- (3) the value that reaches this thread's rows, and the rows
-    A h[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) h[v] = s_in[col * VEC + v];
-    for (int w = 0; w < warp; ++w) {
-      const int wr = s_wreset[w];
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const A a = s_wa[w * C + col * VEC + v], bb = s_wb[w * C + col * VEC + v];
-        h[v] = wr ? bb : apply_map(a, bb, h[v]);
-      }
-    }
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) h[v] = ereset ? eb[v] : apply_map(ea[v], eb[v], h[v]);
-
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int64_t t = row_of(pos0 + r);
-      Mark m{0, 0};
-      if (marked) {
-        m = mark[ty * R + r];
-        if (m.flags & kPad) continue;
-        if (m.flags & (BWD ? kEnd : kStart)) {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) h[v] = 0;
-          if (live) load_acc<A, VEC>(h, p.state, (srow + m.seg) * p.K + c0);
-        }
-      }
-      const bool dead = marked && (m.flags & kDead);
-      const Pack<T, VEC> x = get_src(r, t);
-      const Pack<G, S::kGateVec> g = get_gate(r, t);
-      Pack<T, VEC> o;
-      if constexpr (!BWD) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          h[v] = dead ? (A)0 : to_acc<G>(g.v[SHARED ? 0 : v]) * h[v] + to_acc<T>(x.v[v]);
-          o.v[v] = from_acc<T>(h[v]);
-        }
-        if (live) {
-          st_stream<T, VEC>(out + t * p.K, o);
-          if (marked && (m.flags & kEnd) && p.last) store_acc<A, VEC>(h, p.last, (srow + m.seg) * p.K + c0);
-        }
-      } else {
-        A before[VEC], dg[VEC];
-        if (p.grad_gate) {
-          const Pack<T, VEC> f = S::SrcSlot::get(slot(s_fwd, S::SrcSlot::kBytes, stage, r), fwd + (t - 1) * p.K);
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) before[v] = to_acc<T>(f.v[v]);
-          if (marked && (m.flags & kStart)) {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) before[v] = 0;
-            if (live) load_acc<A, VEC>(before, p.init, (srow + m.seg) * p.K + c0);
-          }
-        }
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const A dh = dead ? (A)0 : h[v] + (p.src ? to_acc<T>(x.v[v]) : (A)0);
-          o.v[v] = from_acc<T>(dh);
-          dg[v] = p.grad_gate && !dead ? dh * before[v] : (A)0;
-          h[v] = dead ? (A)0 : to_acc<G>(g.v[SHARED ? 0 : v]) * dh;
-        }
-        if (live) {
-          st_stream<T, VEC>(out + t * p.K, o);
-          if (marked && (m.flags & kStart) && p.last) store_acc<A, VEC>(h, p.last, (srow + m.seg) * p.K + c0);
-        }
-        if (p.grad_gate) {
-          if constexpr (!SHARED) {
-            Pack<G, VEC> og;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) og.v[v] = from_acc<G>(dg[v]);
-            if (live) st_stream<G, VEC>(static_cast<G *>(p.grad_gate) + (b * p.E + t) * gates + c0, og);
-          } else {
-            // sum of the thread's channels, then of the neighbouring lanes that hold the same gate; the lanes of a row
-            // are in the same iteration together: rows are skipped (kPad) by whole rows
-            A sum = dg[0];
-#pragma unroll
-            for (int v = 1; v < VEC; ++v) sum += dg[v];
-            const unsigned rowmask = (lx == 32 ? kFullMask : ((1u << lx) - 1u) << (lane & ~(lx - 1)));
-            for (int d = 1; d < (1 << p.lanes_log2); d <<= 1) sum += __shfl_xor_sync(rowmask, sum, d);
-            if (live && (col & ((1 << p.lanes_log2) - 1)) == 0) {
-              const int64_t per = VEC << p.lanes_log2;
-              if (per == p.width) static_cast<G *>(p.grad_gate)[(b * p.E + t) * gates + g0] = from_acc<G>(sum);
-              else static_cast<A *>(p.partial)[(b * p.E + t) * (p.K / per) + c0 / per] = sum;
-            }
-          }
-        }
-      }
-    }
+    tile += step;
+    stage = stage == kStages - 1 ? 0 : stage + 1;
+    par ^= 1;
   }
 }
 
@@ -482,7 +524,8 @@ inline unsigned flat_blocks(int64_t items, int per = kThreads) {
 // lanes that hold a row's channels of a tile
 inline int lanes_of_row(int64_t K, int vec, size_t elem) {
   const int wide = vec * elem >= 16 ? 3 : 5;  // 128 bytes of a row, or a whole warp of single values
-  return std::min(wide, ilog2_ceil((K + vec - 1) / vec));
+  // at least four channels: the lanes that share one in step (2) are lanes of one warp
+  return std::min(wide, std::max(ilog2_ceil((K + vec - 1) / vec), vec >= 4 ? 0 : vec == 2 ? 1 : 2));
 }
 // lanes of a row whose gate products a row's shuffles sum: the neighbours that hold the same gate
 inline int lanes_of_gate(int64_t width, int vec, int lx_log2) {
@@ -499,7 +542,7 @@ template <typename T, typename G, int VEC, bool SHARED, bool BWD> int launch_til
   const int lx = 1 << p.lx_log2;
   const int64_t L = (int64_t)(kScanThreads >> p.lx_log2) * S::kRows, C = (int64_t)lx * VEC;
   p.tiles_k = (p.K + C - 1) / C;
-  const int64_t tiles = (p.E + L - 1) / L, want = (int64_t)sm_count() * 3;
+  const int64_t tiles = (p.E + L - 1) / L, want = (int64_t)sm_count() * 2;
   int64_t ctas = p.tiles_k * p.B;
   p.cluster = 1;
   while (p.cluster < kMostCluster && ctas * p.cluster < want && p.cluster * 2 <= tiles) p.cluster *= 2;

@@ -270,22 +270,44 @@ def test_scan(kind, heads, width, states, dtype, gdtype):
 
 
 def test_scan_forms_of_the_gate_agree():
+    """A gate that is shared, expanded, flattened or constant: each form within the roundings of the formula (they are cut
+    into tiles of different lengths, so the bits of two forms need not be the same)."""
     gen = torch.Generator().manual_seed(5)
     E, H, P = 700, 6, 16
-    indptr = torch.tensor([0, 100, 100, 650, 700], device='cuda')
+    ends = [0, 100, 100, 650, 700]
+    indptr = torch.tensor(ends, device='cuda')
     src = rand(gen, E, H, P).cuda()
     gate = torch.rand(E, H, 1, generator=gen).cuda()
-    shared = ts.scan_csr(src, gate, indptr)
-    assert torch.equal(shared, ts.scan_csr(src, gate.expand(E, H, P), indptr))
-    assert torch.equal(shared, ts.scan_csr(src.reshape(E, H * P), gate.expand(E, H, P).reshape(E, H * P), indptr).reshape(E, H, P))
+
+    def bounds(g):
+        h, _, _, mass, way = ref.scan(src.cpu().double().reshape(E, H * P), g.cpu().double().expand(E, H, P).reshape(E, H * P), ends, None)
+        return h, ref.unit(F32) * (4 * way + 32 * mass) + ref.last_rounding(h, F32)
+
+    want, tol = bounds(gate)
+    ref.assert_within(ts.scan_csr(src, gate, indptr).reshape(E, H * P), want, tol, 'shared')
+    ref.assert_within(ts.scan_csr(src, gate.expand(E, H, P), indptr).reshape(E, H * P), want, tol, 'expanded')
+    flat = gate.expand(E, H, P).reshape(E, H * P)
+    ref.assert_within(ts.scan_csr(src.reshape(E, H * P), flat, indptr), want, tol, 'flat')
+
     one = torch.rand(E, 1, 1, generator=gen).cuda().requires_grad_()
     full = one.detach().expand(E, H, P).contiguous().requires_grad_()
+    want, tol = bounds(one.detach())
     a, b = ts.scan_csr(src, one, indptr), ts.scan_csr(src, full, indptr)
-    assert torch.equal(a, b)
-    g = rand(gen, E, H, P).cuda()
-    ga, gb = torch.autograd.grad(a, one, g)[0], torch.autograd.grad(b, full, g)[0]
-    # the sum of H * P products, each within its own rounding, in whatever order
-    ref.assert_within(ga, gb.double().sum((1, 2), keepdim=True).cpu(), (gb.double().abs().sum((1, 2), keepdim=True) * ref.unit(F32) * (H * P + 4)).cpu(), 'gate')
+    ref.assert_within(a.reshape(E, H * P), want, tol, 'one gate')
+    ref.assert_within(b.reshape(E, H * P), want, tol, 'its copies')
+    g = rand(gen, E, H, P)
+    before = torch.roll(want, 1, 0)
+    before[[0, 100, 650]] = 0
+    gates = full.detach().cpu().double().reshape(E, H * P)
+    dh, dg, _, dmass, dway, _, _ = ref.scan_backward(g.double().reshape(E, H * P), None, gates, before, ends)
+    # each product: dh and h within their bounds; then the sum of H * P of them
+    dtol = dh.abs() * torch.roll(tol, 1, 0) + ref.unit(F32) * (4 * dway + 32 * dmass) * before.abs() + 2 * ref.unit(F32) * dg.abs()
+    total = dg.sum(1, keepdim=True)
+    ttol = dtol.sum(1, keepdim=True) + ref.unit(F32) * (H * P + 4) * dg.abs().sum(1, keepdim=True)
+    ga, gb = torch.autograd.grad(a, one, g.cuda())[0], torch.autograd.grad(b, full, g.cuda())[0]
+    ref.assert_within(ga.reshape(E, 1), total, ttol, 'gradient of one gate')
+    ref.assert_within(gb.reshape(E, H * P), dg, dtol, 'gradient of its copies')
+
     decay = torch.rand(P, generator=gen).cuda().reshape(1, 1, P).requires_grad_()  # a constant decay: expanded, gradient summed
     out = ts.scan_csr(src, decay, indptr)
     assert torch.equal(out, ts.scan_csr(src, decay.expand(E, H, P).contiguous(), indptr))
