@@ -22,8 +22,6 @@
 // touches run a copy of the code without these checks.
 #pragma once
 
-#include <cooperative_groups.h>
-
 #include <algorithm>
 #include <atomic>
 
@@ -32,7 +30,7 @@
 namespace tsb {
 namespace scan {
 
-constexpr int kScanThreads = 128;
+constexpr int kScanThreads = 128;           // threads that carry channels; a fifth warp looks for segment borders
 constexpr int kStages = 3;
 constexpr int kMostCluster = 8;
 
@@ -151,6 +149,43 @@ __device__ __forceinline__ int64_t part_begin(const ScanParams &p, const int64_t
   return s <= p.N ? clamp64(indptr[s], 0, p.E) : even;
 }
 
+// ---- exchange between the CTAs of a cluster: values stored into a neighbour's shared memory complete bytes of a barrier
+// there, so a CTA waits for what it needs and for nothing else (a cluster-wide barrier would also wait for the outputs'
+// stores to drain: 1.2 of 7.9 cycles between two instructions of a warp went there)
+__device__ __forceinline__ unsigned smem_at(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ unsigned remote_at(unsigned addr, int rank) {
+  unsigned r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_init(unsigned bar) { asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void mbar_init_done() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+__device__ __forceinline__ void mbar_expect(unsigned bar, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// false if the bytes did not come within the limit (they always do: the CTAs of a cluster run together)
+__device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
+  for (int i = 0; i < (1 << 22); ++i) {
+    unsigned ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ void send(unsigned addr, unsigned bar, float a, float b) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(addr), "f"(a), "f"(b), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void send(unsigned addr, unsigned bar, double a, double b) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f64 [%0], {%1, %2}, [%3];" ::"r"(addr), "d"(a), "d"(b), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void send(unsigned addr, unsigned bar, int v) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(v), "r"(bar) : "memory");
+}
+
 template <typename T, typename G, int VEC, bool SHARED, bool BWD> struct ScanShape {
   using A = acc_t<T>;
   static constexpr int kGateVec = SHARED ? 1 : VEC;
@@ -163,19 +198,18 @@ template <typename T, typename G, int VEC, bool SHARED, bool BWD> struct ScanSha
   static constexpr int kMapBytes = 2 * kScanThreads * VEC * (int)sizeof(A);  // [A, B][ty][C]
   static size_t bytes(int lx, int cluster) {
     const size_t C = (size_t)lx * VEC, L = (size_t)(kScanThreads / lx) * kRows;
-    return (size_t)kStages * kStageBytes + kMapBytes + (cluster > 1 ? sizeof(A) * C * 4 * cluster : 0) + sizeof(int) * 2 * L;
+    return (size_t)kStages * kStageBytes + kMapBytes + (cluster > 1 ? sizeof(A) * C * 4 * cluster : 0) + sizeof(int) * kStages * L;
   }
 };
 
 template <typename T, typename G, int VEC, bool SHARED, bool BWD>
-__global__ void __launch_bounds__(kScanThreads) scan_kernel(ScanParams p) {
+__global__ void __launch_bounds__(kScanThreads + 32) scan_kernel(ScanParams p) {
   using S = ScanShape<T, G, VEC, SHARED, BWD>;
   using SrcSlot = typename S::SrcSlot;
   using GateSlot = typename S::GateSlot;
   using A = acc_t<T>;
   constexpr int R = S::kRows;
   constexpr int kSrcRow = kScanThreads * SrcSlot::kBytes, kGateRow = kScanThreads * GateSlot::kBytes;
-  namespace cg = cooperative_groups;
 
   const int tid = threadIdx.x;
   const int lx = 1 << p.lx_log2, C = lx * VEC, L = (kScanThreads >> p.lx_log2) * R;
@@ -192,79 +226,128 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(ScanParams p) {
   if (len <= 0) return;  // the same for the whole cluster
   const int64_t step = (int64_t)cs * L;
 
+  extern __shared__ __align__(128) char smem[];
+  A *s_a = reinterpret_cast<A *>(smem + (size_t)kStages * S::kStageBytes);  // maps of the threads [ty][C]; then the values
+  A *s_b = s_a + kScanThreads * VEC;                               // that reach them, in place of A
+  A *s_total = s_b + kScanThreads * VEC;                           // maps of the cluster's CTAs [2][cs][C][A, B]
+  int *s_marks = reinterpret_cast<int *>(s_total + (cs > 1 ? 4 * cs * C : 0));  // [stage][L]
+  __shared__ int s_reset[kScanThreads], s_total_reset[2][kMostCluster];
+  __shared__ int s_marked[kStages];                                      // does a segment border touch the tile?
+  __shared__ __align__(8) uint64_t s_bar[2];
+
+  if (cs > 1) {
+    if (tid < 2) {
+      mbar_init(smem_at(&s_bar[tid]));
+      mbar_init_done();
+    }
+    cluster_barrier();  // all CTAs run, with their barriers ready, before anyone writes to their shared memory
+  }
+
+  const auto row_of = [&](int64_t pos) { return BWD ? hi - 1 - pos : lo + pos; };
+
+  // ---- the fifth warp: where segments begin and end, one tile ahead of the others
+  if (tid >= kScanThreads) {
+    const int lane = tid - kScanThreads;
+    int64_t cursor = BWD ? p.N + 1 : 0;  // bound of the last row looked up
+    const auto look = [&](int64_t tile, int stage) {
+      // lane 0 of each search sees the first and the last row of the tile; the same border means none in between
+      const int64_t last = tile + L - 1 < len ? tile + L - 1 : len - 1;
+      const int64_t from = row_of(tile < len ? tile : len - 1), to = row_of(last);
+      const int64_t u = BWD ? bound<true>(indptr, 0, cursor, from) : bound<true>(indptr, cursor, p.N + 1, from);
+      const bool inside = u >= 1 && u <= p.N;
+      const bool whole = tile + L <= len;
+      const bool marked = !(inside && whole && (BWD ? from + 1 < indptr[u] && to > indptr[u - 1] : from > indptr[u - 1] && to + 1 < indptr[u]));
+      cursor = u;
+      if (marked) {
+        for (int j = lane; j < L; j += 32) {
+          const int64_t t = row_of(tile + j < len ? tile + j : len - 1);
+          const int64_t w = BWD ? bound<true>(indptr, 0, u, t) : bound<true>(indptr, u, p.N + 1, t);
+          int flags;
+          if (tile + j >= len) flags = kPad;
+          else if (w < 1 || w > p.N) flags = kDead;
+          else flags = (int)(w - 1) << kMarkBits | (indptr[w - 1] == t ? kStart : 0) | (indptr[w] == t + 1 ? kEnd : 0);
+          s_marks[stage * L + j] = flags;
+        }
+      }
+      if (lane == 0) s_marked[stage] = marked;
+    };
+    int64_t tile = (int64_t)rank * L;
+    int stage = 0;
+    look(tile, 0);
+    __syncthreads();
+    for (int64_t done = 0; done < len; done += step) {
+      tile += step;
+      stage = stage == kStages - 1 ? 0 : stage + 1;
+      if (done + step < len) look(tile, stage);  // of the three stages, the others may still read two
+      __syncthreads();                           // (1) of the tile before is done
+      __syncthreads();                           // (2)
+    }
+    return;
+  }
+
   const int64_t c0 = kt * C + (int64_t)col * VEC;   // this thread's first channel
   const bool live = c0 < p.K;
   const int64_t gates = p.K / p.width, g0 = SHARED ? c0 / p.width : c0;
-  // this thread's pointers to row 0, and the way to its next row
-  const T *src = static_cast<const T *>(p.src) + (p.src ? b * p.E * p.K + c0 : 0);
-  const T *fwd = static_cast<const T *>(p.fwd) + (BWD ? (b * p.E - 1) * p.K + c0 : 0);  // h of the row before
-  const G *gate = static_cast<const G *>(p.gate) + b * p.E * gates + g0;
-  T *out = static_cast<T *>(p.out) + b * p.E * p.K + c0;
-  const int64_t dk = BWD ? -p.K : p.K, dgates = BWD ? -gates : gates;
+  const int64_t dk = BWD ? -p.K : p.K, dgates = BWD ? -gates : gates;  // from a row to the next one on the way
   const int64_t srow = b * p.N;                     // first row of this batch in the state arrays
   const bool have_src = !BWD || p.src, want_gate = BWD && p.grad_gate;
   const T *src_lo = static_cast<const T *>(p.src), *src_hi = src_lo + p.B * p.E * p.K;
   const T *fwd_lo = static_cast<const T *>(p.fwd), *fwd_hi = fwd_lo + p.B * p.E * p.K;
   const G *gate_lo = static_cast<const G *>(p.gate), *gate_hi = gate_lo + p.B * p.E * gates;
 
-  extern __shared__ __align__(128) char smem[];
-  char *s_src = smem + tid * SrcSlot::kBytes;                      // [stage][row][thread], from here on this thread's
+  // this thread's slots [stage][row][thread], and its pointers to the next tile to load and to the tile at work
+  char *s_src = smem + tid * SrcSlot::kBytes;
   char *s_fwd = s_src + kStages * R * kSrcRow;
   char *s_gate = smem + kStages * R * kSrcRow * (BWD ? 2 : 1) + tid * GateSlot::kBytes;
-  A *s_a = reinterpret_cast<A *>(smem + (size_t)kStages * S::kStageBytes);  // maps of the threads [ty][C]; then the values
-  A *s_b = s_a + kScanThreads * VEC;                               // that reach them, in place of A
-  A *s_total = s_b + kScanThreads * VEC;                           // maps of the cluster's CTAs [2][cs][C][A, B]
-  int *s_marks = reinterpret_cast<int *>(s_total + (cs > 1 ? 4 * cs * C : 0));  // [2][L]
-  __shared__ int s_reset[kScanThreads], s_total_reset[2][kMostCluster];
-  __shared__ int64_t s_found[2][2];                                // bound of the tile's last row, next border
+  int64_t tile = (int64_t)rank * L;                 // position of the CTA's tile
+  int64_t ahead = tile + ty * R;                    // position of the thread's next rows to load
+  const int64_t at = b * p.E + row_of(ahead);
+  const T *lsrc = src_lo + (have_src ? at * p.K + c0 : 0), *lfwd = fwd_lo + (BWD ? (at - 1) * p.K + c0 : 0);  // fwd: h of the row before
+  const G *lgate = gate_lo + at * gates + g0;
+  T *os = static_cast<T *>(p.out) + at * p.K + c0;
+  G *og = static_cast<G *>(p.grad_gate) + (want_gate ? at * gates + g0 : 0);
+  const int64_t tile_k = step * dk, tile_gates = step * dgates;
+  // which half of its word a row's value is in (2-byte slots only)
+  const int kodd = (int)(p.K & 1), godd = (int)(gates & 1);
+  int xhalf = SrcSlot::half(lsrc), fhalf = SrcSlot::half(lfwd), ghalf = GateSlot::half(lgate);
+  const int xturn = (int)(tile_k & 1), gturn = (int)(tile_gates & 1);
 
-  if (cs > 1) cg::this_cluster().sync();  // all CTAs run before anyone writes to their shared memory
-
-  const auto row_of = [&](int64_t pos) { return BWD ? hi - 1 - pos : lo + pos; };
-
-  const auto load_tile = [&](int64_t tile, int stage) {
-    const int64_t pos = tile + ty * R;
-    if (live && pos < len) {
-      const int n = (int)(len - pos < R ? len - pos : R);
-      const int64_t t = row_of(pos);
-      const T *xs = src + t * p.K, *fs = fwd + t * p.K;
-      const G *gs = gate + t * gates;
+  const auto load_rows = [&](int stage) {
+    const int64_t left = len - ahead;
+    if (live && left > 0) {
+      const T *xs = lsrc, *fs = lfwd;
+      const G *gs = lgate;
       char *xd = s_src + stage * (R * kSrcRow), *fd = s_fwd + stage * (R * kSrcRow), *gd = s_gate + stage * (R * kGateRow);
-      const auto rows = [&](auto whole) {
+      const int n = left < R ? (int)left : R;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          if (!decltype(whole)::value && r >= n) break;
+      for (int r = 0; r < R; ++r) {
+        if (r < n) {
           if (have_src) SrcSlot::copy(xd + r * kSrcRow, xs, src_lo, src_hi);
           GateSlot::copy(gd + r * kGateRow, gs, gate_lo, gate_hi);
-          if (want_gate && fs >= fwd_lo) SrcSlot::copy(fd + r * kSrcRow, fs, fwd_lo, fwd_hi);  // (row 0 has none before it)
-          xs += dk;
-          fs += dk;
-          gs += dgates;
+          if (BWD && want_gate && fs >= fwd_lo) SrcSlot::copy(fd + r * kSrcRow, fs, fwd_lo, fwd_hi);  // (row 0 has none before it)
         }
-      };
-      if (n == R) rows(std::true_type());
-      else rows(std::false_type());
+        xs += dk;
+        fs += dk;
+        gs += dgates;
+      }
     }
     async_commit();
+    ahead += step;
+    lsrc += tile_k;
+    lfwd += tile_k;
+    lgate += tile_gates;
   };
 
-  // the row that was looked up last: its bound, the next border on the way, whether it is outside
-  int64_t cursor = BWD ? p.N + 1 : 0, border = BWD ? (int64_t)1 << 62 : -1;
-  bool outside = false;
   // (2) runs with the roles turned over: channel fc, the fh-th of H lanes that share it
   const int hbits = 31 - __clz(kScanThreads) - p.lx_log2 - (31 - __clz(VEC)), H = 1 << hbits;
   const int fc = tid >> hbits, fh = tid & (H - 1);
   A carry = 0;  // the value that reaches the cluster's tiles in channel fc
+  unsigned phases = 0;  // parity to wait for, one bit for each of the two barriers
 
-  const auto tile_work = [&](auto has_marks, int64_t tile, int stage, int par) {
+  const auto tile_work = [&](auto has_marks, int stage, int par) {
     constexpr bool MARKED = decltype(has_marks)::value;
-    const int *mark = s_marks + par * L + ty * R;
-    const int64_t t0 = row_of(tile + ty * R);
+    const int *mark = s_marks + stage * L + ty * R;
     const char *xs = s_src + stage * (R * kSrcRow), *fs = s_fwd + stage * (R * kSrcRow), *gs = s_gate + stage * (R * kGateRow);
-    // which half of its word the r-th row's value is in (2-byte slots only)
-    const int xhalf = SrcSlot::half(src + t0 * p.K), fhalf = SrcSlot::half(fwd + t0 * p.K), ghalf = GateSlot::half(gate + t0 * gates);
-    const int kodd = (int)(p.K & 1), godd = (int)(gates & 1);
-
     // ---- (1) the map of this thread's rows
     {
       A ma[VEC], mb[VEC];
@@ -341,19 +424,17 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(ScanParams p) {
     const int wr = MARKED ? __shfl_sync(kFullMask, tr, H - 1, H) : 0;
     A h = carry;
     if (cs > 1) {
-      cg::cluster_group cluster = cg::this_cluster();
-      A *mine = s_total + ((size_t)(par * cs + rank) * C + fc) * 2;
-      for (int q = fh; q < cs; q += H) {
-        A *there = cluster.map_shared_rank(mine, q);
-        there[0] = wa;
-        there[1] = wb;
-      }
-      if (tid < cs) *cluster.map_shared_rank(&s_total_reset[par][rank], tid) = wr;
-      cluster.sync();
+      const unsigned bar = smem_at(&s_bar[par]);
+      if (tid == 0) mbar_expect(bar, (unsigned)(cs * (C * 2 * (int)sizeof(A) + 4)));
+      const unsigned mine = smem_at(s_total + ((par * cs + rank) * C + fc) * 2);
+      for (int q = fh; q < cs; q += H) send(remote_at(mine, q), remote_at(bar, q), wa, wb);
+      if (tid < cs) send(remote_at(smem_at(&s_total_reset[par][rank]), tid), remote_at(bar, tid), wr);
+      if (!mbar_wait(bar, phases >> par & 1)) carry = (A)NAN;
+      phases ^= 1u << par;
       A all = carry;
       for (int q = 0; q < cs; ++q) {
         if (q == rank) h = all;
-        const A *m = s_total + ((size_t)(par * cs + q) * C + fc) * 2;
+        const A *m = s_total + ((par * cs + q) * C + fc) * 2;
         const A a = m[0], bb = m[1];
         all = s_total_reset[par][q] ? bb : apply_map(a, bb, all);
       }
@@ -372,10 +453,10 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(ScanParams p) {
     // ---- (3) the rows, from the value that reaches them
     A v_[VEC];
     take(v_, s_a + tid * VEC);
-    T *os = out + t0 * p.K;
-    int64_t t = t0;
+    T *orow = os;
+    G *grow = og;
 #pragma unroll
-    for (int r = 0; r < R; ++r, os += dk, t += BWD ? -1 : 1) {
+    for (int r = 0; r < R; ++r, orow += dk, grow += dgates) {
       int m = 0;
       if constexpr (MARKED) {
         m = mark[r];
@@ -398,7 +479,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(ScanParams p) {
         }
         round_pack(o, v_);
         if (live) {
-          st_stream<T, VEC>(os, o);
+          st_stream<T, VEC>(orow, o);
           if (MARKED && (m & kEnd) && p.last) store_acc<A, VEC>(v_, p.last, (srow + (m >> kMarkBits)) * p.K + c0);
         }
       } else {
@@ -409,7 +490,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(ScanParams p) {
           if (dead) dh[v] = 0;
         }
         round_pack(o, dh);
-        if (live) st_stream<T, VEC>(os, o);
+        if (live) st_stream<T, VEC>(orow, o);
         if (want_gate) {
           const Pack<T, VEC> f = SrcSlot::get(fs + r * kSrcRow, (fhalf + r * kodd) & 1);
           if (MARKED && (m & kStart)) {
@@ -424,9 +505,9 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(ScanParams p) {
             for (int v = 0; v < VEC; ++v) dg[v] = dead ? (A)0 : dh[v] * to_acc<T>(f.v[v]);
           }
           if constexpr (!SHARED) {
-            Pack<G, VEC> og;
-            round_pack(og, dg);
-            if (live) st_stream<G, VEC>(static_cast<G *>(p.grad_gate) + (b * p.E + t) * gates + c0, og);
+            Pack<G, VEC> q;
+            round_pack(q, dg);
+            if (live) st_stream<G, VEC>(grow, q);
           } else {
             // sum of the thread's channels, then of the neighbouring lanes that hold the same gate; the lanes of a row
             // are here together: rows are skipped (kPad) by whole rows
@@ -437,8 +518,8 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(ScanParams p) {
             for (int d = 1; d < (1 << p.lanes_log2); d <<= 1) sum += __shfl_xor_sync(rowmask, sum, d);
             if (live && (col & ((1 << p.lanes_log2) - 1)) == 0) {
               const int64_t per = VEC << p.lanes_log2;
-              if (per == p.width) static_cast<G *>(p.grad_gate)[(b * p.E + t) * gates + g0] = from_acc<G>(sum);
-              else static_cast<A *>(p.partial)[(b * p.E + t) * (p.K / per) + c0 / per] = sum;
+              if (per == p.width) *grow = from_acc<G>(sum);
+              else static_cast<A *>(p.partial)[(b * p.E + row_of(tile + ty * R + r)) * (p.K / per) + c0 / per] = sum;
             }
           }
         }
@@ -449,48 +530,24 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(ScanParams p) {
     }
   };
 
-  int64_t tile = (int64_t)rank * L, ahead = tile;
-  int stage = 0, ahead_stage = 0, par = 0;
+  int stage = 0, ahead_stage = kStages - 1, par = 0;
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-    load_tile(ahead, ahead_stage);
-    ahead += step;
-    ++ahead_stage;
-  }
+  for (int i = 0; i < kStages - 1; ++i) load_rows(i);
+  __syncthreads();  // the first tile's borders are known
   for (int64_t done = 0; done < len; done += step) {
-    load_tile(ahead, ahead_stage);
-    ahead += step;
-    ahead_stage = ahead_stage == kStages - 1 ? 0 : ahead_stage + 1;
-    // does a border touch this tile: at one of its rows, or right behind its last one?
-    const int64_t edge = BWD ? row_of(tile + L - 1) : row_of(tile) + L;
-    const bool marked = outside || tile + L > len || (BWD ? border >= edge : border <= edge);
-    if (marked) {
-      for (int j = tid; j < L; j += kScanThreads) {
-        const int64_t t = row_of(tile + j < len ? tile + j : len - 1);
-        const int64_t u = BWD ? bound<true>(indptr, 0, cursor, t) : bound<true>(indptr, cursor, p.N + 1, t);
-        int flags;
-        if (tile + j >= len) flags = kPad;
-        else if (u < 1 || u > p.N) flags = kDead;
-        else flags = (int)(u - 1) << kMarkBits | (indptr[u - 1] == t ? kStart : 0) | (indptr[u] == t + 1 ? kEnd : 0);
-        s_marks[par * L + j] = flags;
-        if (j == L - 1) {
-          s_found[par][0] = u;
-          s_found[par][1] = BWD ? (u > 0 ? indptr[u - 1] : -1) : (u <= p.N ? indptr[u] : (int64_t)1 << 62);
-        }
-      }
-    }
+    load_rows(ahead_stage);
+    const bool marked = s_marked[stage];
     async_wait_all_but<kStages - 1>();
-    if (marked) {
-      __syncthreads();
-      cursor = s_found[par][0];
-      border = s_found[par][1];
-      outside = cursor < 1 || cursor > p.N;
-      tile_work(std::true_type(), tile, stage, par);
-    } else {
-      tile_work(std::false_type(), tile, stage, par);
-    }
+    if (marked) tile_work(std::true_type(), stage, par);
+    else tile_work(std::false_type(), stage, par);
     tile += step;
+    os += tile_k;
+    og += tile_gates;
+    xhalf ^= xturn;
+    fhalf ^= xturn;
+    ghalf ^= gturn;
     stage = stage == kStages - 1 ? 0 : stage + 1;
+    ahead_stage = ahead_stage == kStages - 1 ? 0 : ahead_stage + 1;
     par ^= 1;
   }
 }
@@ -559,7 +616,7 @@ template <typename T, typename G, int VEC, bool SHARED, bool BWD> int launch_til
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(ctas * p.parts));
-  cfg.blockDim = dim3(kScanThreads);
+  cfg.blockDim = dim3(kScanThreads + 32);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
