@@ -8,7 +8,7 @@
 //
 // Both are affine maps of the running value, value' = A * value + B, and maps compose: rows are cut into tiles of L rows,
 // and every input is read from HBM once.  A thread owns VEC channels (16 bytes) of R consecutive rows of a tile, which it
-// copies to its own slots of shared memory two tiles ahead (cp.async; nobody else reads them, so the data needs no
+// copies to its own slots of shared memory one tile ahead (cp.async; nobody else reads them, so the data needs no
 // barrier).  (1) It composes its rows' maps and leaves the result in shared memory.  (2) Turned over, a thread takes VEC
 // consecutive maps of one channel, composes them and scans over the lanes that share the channel; the CTAs of a cluster
 // hold neighbouring tiles of the same channels and exchange their totals through distributed shared memory; then the
@@ -31,7 +31,8 @@ namespace tsb {
 namespace scan {
 
 constexpr int kScanThreads = 128;           // threads that carry channels; a fifth warp looks for segment borders
-constexpr int kStages = 3;
+constexpr int kStages = 2;
+constexpr int kMarkStages = 3;
 constexpr int kMostCluster = 8;
 
 struct ScanParams {
@@ -111,6 +112,56 @@ template <typename A, int VEC> __device__ __forceinline__ void take(A (&v)[VEC],
   }
 }
 
+// A pack in the accumulation type: a bf16 value is the upper half of the fp32 value, so two come out of a word with a
+// shift and a mask.
+template <typename T, int VEC, typename A> __device__ __forceinline__ void widen(A (&v)[VEC], const Pack<T, VEC> &q) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value && VEC % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      const unsigned w = *reinterpret_cast<const unsigned *>(&q.v[i]);
+      v[i] = __uint_as_float(w << 16);
+      v[i + 1] = __uint_as_float(w & 0xffff0000u);
+    }
+  } else if constexpr (std::is_same<T, __half>::value && VEC % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&q.v[i]));
+      v[i] = f.x;
+      v[i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = to_acc<T>(q.v[i]);
+  }
+}
+
+// a * b + c, a * b and a + b over VEC channels, two fp32 channels in one instruction
+template <typename A, int VEC, typename F2, typename F1> __device__ __forceinline__ void pairwise(A (&d)[VEC], F2 two, F1 one) {
+  if constexpr (std::is_same<A, float>::value && VEC % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      const float2 r = two(i);
+      d[i] = r.x;
+      d[i + 1] = r.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) d[i] = one(i);
+  }
+}
+template <typename A, int VEC> __device__ __forceinline__ void fma_all(A (&d)[VEC], const A (&a)[VEC], const A (&b)[VEC], const A (&c)[VEC]) {
+  pairwise<A, VEC>(d, [&](int i) { return __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]), make_float2(c[i], c[i + 1])); },
+                   [&](int i) { return a[i] * b[i] + c[i]; });
+}
+template <typename A, int VEC> __device__ __forceinline__ void mul_all(A (&d)[VEC], const A (&a)[VEC], const A (&b)[VEC]) {
+  pairwise<A, VEC>(d, [&](int i) { return __fmul2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1])); },
+                   [&](int i) { return a[i] * b[i]; });
+}
+template <typename A, int VEC> __device__ __forceinline__ void add_all(A (&d)[VEC], const A (&a)[VEC], const A (&b)[VEC]) {
+  pairwise<A, VEC>(d, [&](int i) { return __fadd2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1])); },
+                   [&](int i) { return a[i] + b[i]; });
+}
+
 // Round to the output's type, once; pairs of 16-bit values in one instruction.
 template <typename T, int VEC, typename A> __device__ __forceinline__ void round_pack(Pack<T, VEC> &o, const A (&v)[VEC]) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value && VEC % 2 == 0) {
@@ -125,8 +176,19 @@ template <typename T, int VEC, typename A> __device__ __forceinline__ void round
   }
 }
 
-// A * h + B.  The product of a tile's gates may overflow where the recurrence itself stays at zero.
-template <typename A> __device__ __forceinline__ A apply_map(A a, A b, A h) { return h == (A)0 ? b : a * h + b; }
+// A product of gates may overflow where the recurrence itself stays at zero: kept finite, so that A * 0 + B = B.
+template <typename A> __device__ __forceinline__ A finite(A a) {
+  constexpr A most = std::numeric_limits<A>::max();
+  return a > most ? most : a < -most ? -most : a;
+}
+
+// A map that drops what comes in travels between CTAs with this A, which no product of gates can be.
+template <typename A> __device__ __forceinline__ A reset_mark() {
+  if constexpr (sizeof(A) == 8) return __longlong_as_double(0x7ff8c0dec0dec0deLL);
+  else return __int_as_float(0x7fc0c0de);
+}
+__device__ __forceinline__ bool is_reset_mark(float a) { return __float_as_int(a) == 0x7fc0c0de; }
+__device__ __forceinline__ bool is_reset_mark(double a) { return __double_as_longlong(a) == 0x7ff8c0dec0dec0deLL; }
 
 // first index in [lo, hi) with indptr[index] > row (UPPER) or >= row; hi if there is none
 template <bool UPPER> __device__ __forceinline__ int64_t bound(const int64_t *indptr, int64_t lo, int64_t hi, int64_t row) {
@@ -182,28 +244,28 @@ __device__ __forceinline__ void send(unsigned addr, unsigned bar, float a, float
 __device__ __forceinline__ void send(unsigned addr, unsigned bar, double a, double b) {
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f64 [%0], {%1, %2}, [%3];" ::"r"(addr), "d"(a), "d"(b), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void send(unsigned addr, unsigned bar, int v) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(v), "r"(bar) : "memory");
-}
-
 template <typename T, typename G, int VEC, bool SHARED, bool BWD> struct ScanShape {
   using A = acc_t<T>;
   static constexpr int kGateVec = SHARED ? 1 : VEC;
   using SrcSlot = Slot<T, VEC>;
   using GateSlot = Slot<G, kGateVec>;
   static constexpr int kRowBytes = SrcSlot::kBytes * (BWD ? 2 : 1) + GateSlot::kBytes;
-  // rows of a thread: 28 KB for each of the three stages at most, so that two CTAs and more fit an SM
-  static constexpr int kRows = 224 / kRowBytes < 16 ? 224 / kRowBytes : 16;
+  // Rows of a thread: 42 KB for each of the two stages at most, so that two CTAs fit an SM.  What a tile costs besides its
+  // rows, step (2), is then a small part (65536 x 4096 bf16: 291 us with 10 rows and 2 stages, 302 with 7 rows and 3
+  // stages, 391 with 5 rows, 2 stages and four CTAs).
+  static constexpr int kRows = 336 / kRowBytes < 16 ? 336 / kRowBytes : 16;
+  static constexpr int kCtas = kRowBytes <= 16 ? 4 : 2;  // of an SM, by the registers
   static constexpr int kStageBytes = kScanThreads * kRows * kRowBytes;
-  static constexpr int kMapBytes = 2 * kScanThreads * VEC * (int)sizeof(A);  // [A, B][ty][C]
+  static constexpr int kMaps = kScanThreads * VEC + 128;      // [ty][C], see `skew`
+  static constexpr int kMapBytes = 2 * kMaps * (int)sizeof(A);
   static size_t bytes(int lx, int cluster) {
     const size_t C = (size_t)lx * VEC, L = (size_t)(kScanThreads / lx) * kRows;
-    return (size_t)kStages * kStageBytes + kMapBytes + (cluster > 1 ? sizeof(A) * C * 4 * cluster : 0) + sizeof(int) * kStages * L;
+    return (size_t)kStages * kStageBytes + kMapBytes + (cluster > 1 ? sizeof(A) * C * 4 * cluster : 0) + sizeof(int) * kMarkStages * L;
   }
 };
 
 template <typename T, typename G, int VEC, bool SHARED, bool BWD>
-__global__ void __launch_bounds__(kScanThreads + 32) scan_kernel(ScanParams p) {
+__global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED, BWD>::kCtas) scan_kernel(ScanParams p) {
   using S = ScanShape<T, G, VEC, SHARED, BWD>;
   using SrcSlot = typename S::SrcSlot;
   using GateSlot = typename S::GateSlot;
@@ -228,11 +290,11 @@ __global__ void __launch_bounds__(kScanThreads + 32) scan_kernel(ScanParams p) {
 
   extern __shared__ __align__(128) char smem[];
   A *s_a = reinterpret_cast<A *>(smem + (size_t)kStages * S::kStageBytes);  // maps of the threads [ty][C]; then the values
-  A *s_b = s_a + kScanThreads * VEC;                               // that reach them, in place of A
-  A *s_total = s_b + kScanThreads * VEC;                           // maps of the cluster's CTAs [2][cs][C][A, B]
+  A *s_b = s_a + S::kMaps;                                         // that reach them, in place of A
+  A *s_total = s_b + S::kMaps;                           // maps of the cluster's CTAs [2][cs][C][A, B]
   int *s_marks = reinterpret_cast<int *>(s_total + (cs > 1 ? 4 * cs * C : 0));  // [stage][L]
-  __shared__ int s_reset[kScanThreads], s_total_reset[2][kMostCluster];
-  __shared__ int s_marked[kStages];                                      // does a segment border touch the tile?
+  __shared__ int s_reset[kScanThreads];
+  __shared__ int s_marked[kMarkStages];                                      // does a segment border touch the tile?
   __shared__ __align__(8) uint64_t s_bar[2];
 
   if (cs > 1) {
@@ -248,28 +310,38 @@ __global__ void __launch_bounds__(kScanThreads + 32) scan_kernel(ScanParams p) {
   // ---- the fifth warp: where segments begin and end, one tile ahead of the others
   if (tid >= kScanThreads) {
     const int lane = tid - kScanThreads;
-    int64_t cursor = BWD ? p.N + 1 : 0;  // bound of the last row looked up
+    const int64_t first = indptr[0], behind = indptr[p.N];
+    int64_t cursor = BWD ? p.N + 1 : 0;  // bound of the row looked up last
     const auto look = [&](int64_t tile, int stage) {
-      // lane 0 of each search sees the first and the last row of the tile; the same border means none in between
-      const int64_t last = tile + L - 1 < len ? tile + L - 1 : len - 1;
-      const int64_t from = row_of(tile < len ? tile : len - 1), to = row_of(last);
+      // the segment of the tile's first row on the way: does it hold the whole tile, without beginning or ending in it?
+      const int64_t from = row_of(tile < len ? tile : len - 1), to = row_of(tile + L <= len ? tile + L - 1 : len - 1);
       const int64_t u = BWD ? bound<true>(indptr, 0, cursor, from) : bound<true>(indptr, cursor, p.N + 1, from);
-      const bool inside = u >= 1 && u <= p.N;
-      const bool whole = tile + L <= len;
-      const bool marked = !(inside && whole && (BWD ? from + 1 < indptr[u] && to > indptr[u - 1] : from > indptr[u - 1] && to + 1 < indptr[u]));
       cursor = u;
-      if (marked) {
+      const int64_t low = BWD ? to : from, high = BWD ? from : to;
+      const bool plain = tile + L <= len && u >= 1 && u <= p.N && indptr[u - 1] < low && indptr[u] > high + 1;
+      if (!plain) {
+        int *mark = s_marks + stage * L;
         for (int j = lane; j < L; j += 32) {
-          const int64_t t = row_of(tile + j < len ? tile + j : len - 1);
-          const int64_t w = BWD ? bound<true>(indptr, 0, u, t) : bound<true>(indptr, u, p.N + 1, t);
-          int flags;
-          if (tile + j >= len) flags = kPad;
-          else if (w < 1 || w > p.N) flags = kDead;
-          else flags = (int)(w - 1) << kMarkBits | (indptr[w - 1] == t ? kStart : 0) | (indptr[w] == t + 1 ? kEnd : 0);
-          s_marks[stage * L + j] = flags;
+          const int64_t t = row_of(tile + j);
+          mark[j] = tile + j >= len ? kPad : t < first || t >= behind ? kDead : 0;
+        }
+        __syncwarp();
+        // borders from the first row's segment on, 32 at a time, until one is beyond the tile
+        for (int64_t s0 = BWD ? u : u - 1;; s0 += BWD ? -32 : 32) {
+          const int64_t s = BWD ? s0 - lane : s0 + lane;
+          bool beyond = s < 0 || s > p.N;
+          if (!beyond) {
+            const int64_t at = indptr[s];
+            beyond = BWD ? at < low : at > high + 1;
+            if (at >= low && at <= high && s < p.N && indptr[s + 1] > at)
+              atomicOr(&mark[BWD ? high - at : at - low], (int)s << kMarkBits | kStart);
+            if (at > low && at <= high + 1 && s > 0 && indptr[s - 1] < at)
+              atomicOr(&mark[BWD ? high - (at - 1) : at - 1 - low], (int)(s - 1) << kMarkBits | kEnd);
+          }
+          if (__any_sync(kFullMask, beyond && (BWD ? s <= p.N : s >= 0))) break;
         }
       }
-      if (lane == 0) s_marked[stage] = marked;
+      if (lane == 0) s_marked[stage] = !plain;
     };
     int64_t tile = (int64_t)rank * L;
     int stage = 0;
@@ -277,8 +349,8 @@ __global__ void __launch_bounds__(kScanThreads + 32) scan_kernel(ScanParams p) {
     __syncthreads();
     for (int64_t done = 0; done < len; done += step) {
       tile += step;
-      stage = stage == kStages - 1 ? 0 : stage + 1;
-      if (done + step < len) look(tile, stage);  // of the three stages, the others may still read two
+      stage = stage == kMarkStages - 1 ? 0 : stage + 1;
+      if (done + step < len) look(tile, stage);  // of the three sets of marks, the others may still read two
       __syncthreads();                           // (1) of the tile before is done
       __syncthreads();                           // (2)
     }
@@ -306,6 +378,11 @@ __global__ void __launch_bounds__(kScanThreads + 32) scan_kernel(ScanParams p) {
   const G *lgate = gate_lo + at * gates + g0;
   T *os = static_cast<T *>(p.out) + at * p.K + c0;
   G *og = static_cast<G *>(p.grad_gate) + (want_gate ? at * gates + g0 : 0);
+  // sums of a shared gate's products: all of them, or what this tile's lanes hold
+  const int sum_lanes = SHARED ? 1 << p.lanes_log2 : 1;
+  const int64_t sums = SHARED ? p.K / ((int64_t)VEC * sum_lanes) : 0, dsums = BWD ? -sums : sums;
+  const bool part_sums = SHARED && sums != gates;
+  A *op = static_cast<A *>(p.partial) + (part_sums && want_gate ? at * sums + c0 / ((int64_t)VEC * sum_lanes) : 0);
   const int64_t tile_k = step * dk, tile_gates = step * dgates;
   // which half of its word a row's value is in (2-byte slots only)
   const int kodd = (int)(p.K & 1), godd = (int)(gates & 1);
@@ -341,15 +418,39 @@ __global__ void __launch_bounds__(kScanThreads + 32) scan_kernel(ScanParams p) {
   // (2) runs with the roles turned over: channel fc, the fh-th of H lanes that share it
   const int hbits = 31 - __clz(kScanThreads) - p.lx_log2 - (31 - __clz(VEC)), H = 1 << hbits;
   const int fc = tid >> hbits, fh = tid & (H - 1);
+  // the H lanes of a channel read maps VEC * C apart, all in one bank: each VEC rows of maps start some words further on
+  const int skew = H > 8 ? 4 : 32 >> hbits;
   A carry = 0;  // the value that reaches the cluster's tiles in channel fc
+  const int own_map = tid * VEC + (H > 1 ? ty / VEC * skew : 0), first_map = fh * VEC * C + fc + (H > 1 ? fh * skew : 0);
   unsigned phases = 0;  // parity to wait for, one bit for each of the two barriers
 
-  const auto tile_work = [&](auto has_marks, int stage, int par) {
-    constexpr bool MARKED = decltype(has_marks)::value;
-    const int *mark = s_marks + stage * L + ty * R;
-    const char *xs = s_src + stage * (R * kSrcRow), *fs = s_fwd + stage * (R * kSrcRow), *gs = s_gate + stage * (R * kGateRow);
+  const auto tile_work = [&](int stage, int par, int set) {
+    // does a border touch the tile, and this warp's rows?
+    const bool marked = s_marked[set];
+    const int *mark = s_marks + set * L + ty * R;
+    bool mine = false;
+    if (marked) {
+      int any = 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) any |= mark[r];
+      mine = __any_sync(kFullMask, any != 0);
+    }
+    const char *xs = s_src + stage * (R * kSrcRow), *gs = s_gate + stage * (R * kGateRow);
+    [[maybe_unused]] const char *fs = s_fwd + stage * (R * kSrcRow);
+    const auto read_row = [&](A (&x)[VEC], A (&g)[VEC], int r) {
+      widen<T, VEC>(x, SrcSlot::get(xs + r * kSrcRow, (xhalf + r * kodd) & 1));
+      if constexpr (SHARED) {
+        const A one = to_acc<G>(GateSlot::get(gs + r * kGateRow, (ghalf + r * godd) & 1).v[0]);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) g[v] = one;
+      } else {
+        widen<G, VEC>(g, GateSlot::get(gs + r * kGateRow, (ghalf + r * godd) & 1));
+      }
+    };
+
     // ---- (1) the map of this thread's rows
-    {
+    const auto map_rows = [&](auto has_marks) {
+      constexpr bool MARKED = decltype(has_marks)::value;
       A ma[VEC], mb[VEC];
 #pragma unroll
       for (int v = 0; v < VEC; ++v) { ma[v] = 1; mb[v] = 0; }
@@ -367,25 +468,30 @@ __global__ void __launch_bounds__(kScanThreads + 32) scan_kernel(ScanParams p) {
             if (live) load_acc<A, VEC>(mb, p.state, (srow + (m >> kMarkBits)) * p.K + c0);
           }
         }
-        const Pack<T, VEC> x = SrcSlot::get(xs + r * kSrcRow, (xhalf + r * kodd) & 1);
-        const Pack<G, S::kGateVec> g = GateSlot::get(gs + r * kGateRow, (ghalf + r * godd) & 1);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const A gv = to_acc<G>(g.v[SHARED ? 0 : v]);
-          if constexpr (BWD) mb[v] = gv * (have_src ? mb[v] + to_acc<T>(x.v[v]) : mb[v]);
-          else mb[v] = gv * mb[v] + to_acc<T>(x.v[v]);
-          if (!SHARED || v == 0) ma[v] *= gv;
+        A x[VEC], g[VEC];
+        read_row(x, g, r);
+        if constexpr (BWD) {
+          if (have_src) add_all(mb, mb, x);
+          mul_all(mb, g, mb);
+        } else {
+          fma_all(mb, g, mb, x);
         }
+        if constexpr (SHARED) ma[0] *= g[0];
+        else mul_all(ma, ma, g);
       }
-      A *pa = s_a + tid * VEC, *pb = s_b + tid * VEC;
+      A *pa = s_a + own_map, *pb = s_b + own_map;
       if constexpr (SHARED) {
 #pragma unroll
         for (int v = 1; v < VEC; ++v) ma[v] = ma[0];
       }
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) ma[v] = finite(ma[v]);
       put(pa, ma);
       put(pb, mb);
-      if (MARKED && col == 0) s_reset[ty] = reset;
-    }
+      if (marked && col == 0) s_reset[ty] = reset;
+    };
+    if (mine) map_rows(std::true_type());
+    else map_rows(std::false_type());
     __syncthreads();
 
     // ---- (2) scan of the maps over the tile and the cluster
@@ -393,42 +499,41 @@ __global__ void __launch_bounds__(kScanThreads + 32) scan_kernel(ScanParams p) {
     unsigned fr = 0;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      const int at = (fh * VEC + j) * C + fc;
-      fa[j] = s_a[at];
-      fb[j] = s_b[at];
-      if (MARKED) fr |= (unsigned)s_reset[fh * VEC + j] << j;
+      fa[j] = s_a[first_map + j * C];
+      fb[j] = s_b[first_map + j * C];
+      if (marked) fr |= (unsigned)s_reset[fh * VEC + j] << j;
     }
     A ta = fa[0], tb = fb[0];
     int tr = fr & 1;
 #pragma unroll
     for (int j = 1; j < VEC; ++j) {
-      const bool rs = MARKED && (fr >> j & 1);
-      tb = rs ? fb[j] : apply_map(fa[j], fb[j], tb);
+      const bool rs = marked && (fr >> j & 1);
+      tb = rs ? fb[j] : fa[j] * tb + fb[j];
       ta *= fa[j];
       tr |= rs;
     }
+    ta = finite(ta);
     for (int d = 1; d < H; d <<= 1) {
       const A pa = __shfl_up_sync(kFullMask, ta, d, H), pb = __shfl_up_sync(kFullMask, tb, d, H);
-      const int pr = MARKED ? __shfl_up_sync(kFullMask, tr, d, H) : 0;
+      const int pr = marked ? __shfl_up_sync(kFullMask, tr, d, H) : 0;
       if (fh >= d) {
-        if (!MARKED || !tr) tb = apply_map(ta, tb, pb);
-        ta *= pa;
+        if (!tr) tb = ta * pb + tb;
+        ta = finite(ta * pa);
         tr |= pr;
       }
     }
     // map of the lanes before this one
     const A ea = __shfl_up_sync(kFullMask, ta, 1, H), eb = __shfl_up_sync(kFullMask, tb, 1, H);
-    const int er = MARKED ? __shfl_up_sync(kFullMask, tr, 1, H) : 0;
+    const int er = marked ? __shfl_up_sync(kFullMask, tr, 1, H) : 0;
     // map of the whole tile
     const A wa = __shfl_sync(kFullMask, ta, H - 1, H), wb = __shfl_sync(kFullMask, tb, H - 1, H);
-    const int wr = MARKED ? __shfl_sync(kFullMask, tr, H - 1, H) : 0;
+    const int wr = marked ? __shfl_sync(kFullMask, tr, H - 1, H) : 0;
     A h = carry;
     if (cs > 1) {
       const unsigned bar = smem_at(&s_bar[par]);
-      if (tid == 0) mbar_expect(bar, (unsigned)(cs * (C * 2 * (int)sizeof(A) + 4)));
+      if (tid == 0) mbar_expect(bar, (unsigned)(cs * C * 2 * (int)sizeof(A)));
       const unsigned mine = smem_at(s_total + ((par * cs + rank) * C + fc) * 2);
-      for (int q = fh; q < cs; q += H) send(remote_at(mine, q), remote_at(bar, q), wa, wb);
-      if (tid < cs) send(remote_at(smem_at(&s_total_reset[par][rank]), tid), remote_at(bar, tid), wr);
+      for (int q = fh; q < cs; q += H) send(remote_at(mine, q), remote_at(bar, q), wr ? reset_mark<A>() : wa, wb);
       if (!mbar_wait(bar, phases >> par & 1)) carry = (A)NAN;
       phases ^= 1u << par;
       A all = carry;
@@ -436,27 +541,30 @@ __global__ void __launch_bounds__(kScanThreads + 32) scan_kernel(ScanParams p) {
         if (q == rank) h = all;
         const A *m = s_total + ((par * cs + q) * C + fc) * 2;
         const A a = m[0], bb = m[1];
-        all = s_total_reset[par][q] ? bb : apply_map(a, bb, all);
+        all = is_reset_mark(a) ? bb : a * all + bb;
       }
       carry = all;
     } else {
-      carry = wr ? wb : apply_map(wa, wb, carry);
+      carry = wr ? wb : wa * carry + wb;
     }
-    if (fh > 0) h = er ? eb : apply_map(ea, eb, h);
+    if (fh > 0) h = er ? eb : ea * h + eb;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      s_a[(fh * VEC + j) * C + fc] = h;
-      h = MARKED && (fr >> j & 1) ? fb[j] : apply_map(fa[j], fb[j], h);
+      s_a[first_map + j * C] = h;
+      h = marked && (fr >> j & 1) ? fb[j] : fa[j] * h + fb[j];
     }
     __syncthreads();
 
     // ---- (3) the rows, from the value that reaches them
+    const auto write_rows = [&](auto has_marks) {
+    constexpr bool MARKED = decltype(has_marks)::value;
     A v_[VEC];
-    take(v_, s_a + tid * VEC);
+    take(v_, s_a + own_map);
     T *orow = os;
     G *grow = og;
+    A *prow = op;
 #pragma unroll
-    for (int r = 0; r < R; ++r, orow += dk, grow += dgates) {
+    for (int r = 0; r < R; ++r, orow += dk, grow += dgates, prow += dsums) {
       int m = 0;
       if constexpr (MARKED) {
         m = mark[r];
@@ -468,14 +576,14 @@ __global__ void __launch_bounds__(kScanThreads + 32) scan_kernel(ScanParams p) {
         }
       }
       const bool dead = MARKED && (m & kDead);
-      const Pack<T, VEC> x = SrcSlot::get(xs + r * kSrcRow, (xhalf + r * kodd) & 1);
-      const Pack<G, S::kGateVec> g = GateSlot::get(gs + r * kGateRow, (ghalf + r * godd) & 1);
+      A x[VEC], g[VEC];
+      read_row(x, g, r);
       Pack<T, VEC> o;
       if constexpr (!BWD) {
+        fma_all(v_, g, v_, x);
+        if (dead) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          v_[v] = to_acc<G>(g.v[SHARED ? 0 : v]) * v_[v] + to_acc<T>(x.v[v]);
-          if (dead) v_[v] = 0;
+          for (int v = 0; v < VEC; ++v) v_[v] = 0;
         }
         round_pack(o, v_);
         if (live) {
@@ -485,25 +593,23 @@ __global__ void __launch_bounds__(kScanThreads + 32) scan_kernel(ScanParams p) {
       } else {
         A dh[VEC], dg[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          dh[v] = have_src ? v_[v] + to_acc<T>(x.v[v]) : v_[v];
-          if (dead) dh[v] = 0;
+        for (int v = 0; v < VEC; ++v) dh[v] = v_[v];
+        if (have_src) add_all(dh, v_, x);
+        if (dead) {
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) dh[v] = 0;
         }
         round_pack(o, dh);
         if (live) st_stream<T, VEC>(orow, o);
         if (want_gate) {
-          const Pack<T, VEC> f = SrcSlot::get(fs + r * kSrcRow, (fhalf + r * kodd) & 1);
-          if (MARKED && (m & kStart)) {
-            A before[VEC];
+          A before[VEC];
+          widen<T, VEC>(before, SrcSlot::get(fs + r * kSrcRow, (fhalf + r * kodd) & 1));
+          if (MARKED && (m & (kStart | kDead))) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) before[v] = 0;
-            if (live) load_acc<A, VEC>(before, p.init, (srow + (m >> kMarkBits)) * p.K + c0);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) dg[v] = dh[v] * before[v];
-          } else {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) dg[v] = dead ? (A)0 : dh[v] * to_acc<T>(f.v[v]);
+            if (live && (m & kStart)) load_acc<A, VEC>(before, p.init, (srow + (m >> kMarkBits)) * p.K + c0);
           }
+          mul_all(dg, dh, before);
           if constexpr (!SHARED) {
             Pack<G, VEC> q;
             round_pack(q, dg);
@@ -515,39 +621,44 @@ __global__ void __launch_bounds__(kScanThreads + 32) scan_kernel(ScanParams p) {
 #pragma unroll
             for (int v = 1; v < VEC; ++v) sum += dg[v];
             const unsigned rowmask = lx == 32 ? kFullMask : ((1u << lx) - 1u) << ((tid & 31) & ~(lx - 1));
-            for (int d = 1; d < (1 << p.lanes_log2); d <<= 1) sum += __shfl_xor_sync(rowmask, sum, d);
-            if (live && (col & ((1 << p.lanes_log2) - 1)) == 0) {
-              const int64_t per = VEC << p.lanes_log2;
-              if (per == p.width) *grow = from_acc<G>(sum);
-              else static_cast<A *>(p.partial)[(b * p.E + row_of(tile + ty * R + r)) * (p.K / per) + c0 / per] = sum;
+            for (int d = 1; d < sum_lanes; d <<= 1) sum += __shfl_xor_sync(rowmask, sum, d);
+            if (live && (col & (sum_lanes - 1)) == 0) {
+              if (part_sums) *prow = sum;
+              else *grow = from_acc<G>(sum);
             }
           }
         }
+        mul_all(v_, g, dh);
+        if (dead) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) v_[v] = dead ? (A)0 : to_acc<G>(g.v[SHARED ? 0 : v]) * dh[v];
+          for (int v = 0; v < VEC; ++v) v_[v] = 0;
+        }
         if (MARKED && live && (m & kStart) && p.last) store_acc<A, VEC>(v_, p.last, (srow + (m >> kMarkBits)) * p.K + c0);
       }
     }
+    };
+    if (mine) write_rows(std::true_type());
+    else write_rows(std::false_type());
   };
 
-  int stage = 0, ahead_stage = kStages - 1, par = 0;
+  int stage = 0, ahead_stage = kStages - 1, par = 0, set = 0;
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) load_rows(i);
   __syncthreads();  // the first tile's borders are known
   for (int64_t done = 0; done < len; done += step) {
     load_rows(ahead_stage);
-    const bool marked = s_marked[stage];
     async_wait_all_but<kStages - 1>();
-    if (marked) tile_work(std::true_type(), stage, par);
-    else tile_work(std::false_type(), stage, par);
+    tile_work(stage, par, set);
     tile += step;
     os += tile_k;
     og += tile_gates;
+    op += step * dsums;
     xhalf ^= xturn;
     fhalf ^= xturn;
     ghalf ^= gturn;
     stage = stage == kStages - 1 ? 0 : stage + 1;
     ahead_stage = ahead_stage == kStages - 1 ? 0 : ahead_stage + 1;
+    set = set == kMarkStages - 1 ? 0 : set + 1;
     par ^= 1;
   }
 }
@@ -578,11 +689,12 @@ inline unsigned flat_blocks(int64_t items, int per = kThreads) {
   return (unsigned)std::max<int64_t>(1, std::min<int64_t>((items + per - 1) / per, (int64_t)sm_count() * 32));
 }
 
-// lanes that hold a row's channels of a tile
+// At least four channels: the lanes that share one in step (2) have to be lanes of one warp.
+inline int least_lanes(int vec) { return vec >= 4 ? 0 : vec == 2 ? 1 : 2; }
+// lanes that hold a row's channels of a tile, at most
 inline int lanes_of_row(int64_t K, int vec, size_t elem) {
   const int wide = vec * elem >= 16 ? 3 : 5;  // 128 bytes of a row, or a whole warp of single values
-  // at least four channels: the lanes that share one in step (2) are lanes of one warp
-  return std::min(wide, std::max(ilog2_ceil((K + vec - 1) / vec), vec >= 4 ? 0 : vec == 2 ? 1 : 2));
+  return std::min(wide, std::max(ilog2_ceil((K + vec - 1) / vec), least_lanes(vec)));
 }
 // lanes of a row whose gate products a row's shuffles sum: the neighbours that hold the same gate
 inline int lanes_of_gate(int64_t width, int vec, int lx_log2) {
@@ -594,28 +706,48 @@ inline int lanes_of_gate(int64_t width, int vec, int lx_log2) {
 template <typename T, typename G, int VEC, bool SHARED, bool BWD> int launch_tiles(ScanParams p, cudaStream_t stream) {
   using S = ScanShape<T, G, VEC, SHARED, BWD>;
   auto kernel = scan_kernel<T, G, VEC, SHARED, BWD>;
-  p.lx_log2 = lanes_of_row(p.K, VEC, sizeof(T));
-  p.lanes_log2 = SHARED ? lanes_of_gate(p.width, VEC, p.lx_log2) : 0;
-  const int lx = 1 << p.lx_log2;
-  const int64_t L = (int64_t)(kScanThreads >> p.lx_log2) * S::kRows, C = (int64_t)lx * VEC;
-  p.tiles_k = (p.K + C - 1) / C;
-  const int64_t tiles = (p.E + L - 1) / L, want = (int64_t)sm_count() * 2;
-  int64_t ctas = p.tiles_k * p.B;
-  p.cluster = 1;
-  while (p.cluster < kMostCluster && ctas * p.cluster < want && p.cluster * 2 <= tiles) p.cluster *= 2;
-  ctas *= p.cluster;
-  p.parts = std::max<int64_t>(1, std::min<int64_t>({want / ctas, p.N, tiles / p.cluster}));
-  if (ctas * p.parts > 2147483647LL) return TSB_ERR_TOO_LARGE;
-  const size_t bytes = S::bytes(lx, p.cluster);
-  static std::atomic<int> allowed[64];
+  static std::atomic<int> resident[64][8];  // CTAs of an SM by the lanes of a row; also: the attributes are set
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TSB_ERR_LAUNCH;
-  if (allowed[dev].load() == 0) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) return TSB_ERR_LAUNCH;
-    allowed[dev].store(1);
+  const auto ctas_of_sm = [&](int lx_log2) -> int {
+    int n = resident[dev][lx_log2].load();
+    if (n == 0) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess ||
+          cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kScanThreads + 32, S::bytes(1 << lx_log2, kMostCluster)) != cudaSuccess || n < 1)
+        return 0;
+      resident[dev][lx_log2].store(n);
+    }
+    return n;
+  };
+  // Work is spread over as many CTAs as the GPU holds.  Rows are cut into parts at segment borders where there are
+  // segments enough (six to a part make parts of similar length), and over a cluster for the rest, since
+  // its CTAs wait for each other at every tile: 37 segments over 65536 x 2048 bf16 take 199 us with a cluster of 8 and
+  // one part, 174 with 2 and 4, 179 with 1 and 9.  Where that leaves half the GPU empty a tile gets fewer channels (down
+  // to 32 bytes of a row) and more rows: one segment of 65536 x 1024 takes 139 us at 128 bytes of a row, 98 at 64 and 141
+  // at 32, which no longer fit at once.
+  int64_t ctas = 0;
+  p.lx_log2 = lanes_of_row(p.K, VEC, sizeof(T));
+  for (;;) {
+    const int64_t C = (int64_t)VEC << p.lx_log2, L = (int64_t)(kScanThreads >> p.lx_log2) * S::kRows;
+    p.tiles_k = (p.K + C - 1) / C;
+    const int64_t tiles = (p.E + L - 1) / L, want = (int64_t)sm_count() * ctas_of_sm(p.lx_log2);
+    if (want == 0) return TSB_ERR_LAUNCH;
+    ctas = p.tiles_k * p.B;
+    const int64_t even_parts = std::max<int64_t>(1, p.N / 6);
+    p.cluster = 1;
+    while (p.cluster < kMostCluster && ctas * p.cluster * even_parts < want && p.cluster * 2 <= tiles) p.cluster *= 2;
+    ctas *= p.cluster;
+    p.parts = std::max<int64_t>(1, std::min<int64_t>({want / ctas, p.N, tiles / p.cluster}));
+    ctas *= p.parts;
+    if (ctas * 2 > want || p.lx_log2 <= least_lanes(VEC) || C * (int64_t)sizeof(T) <= 32 || tiles < 2 * p.cluster * p.parts) break;
+    --p.lx_log2;
   }
+  const int lx = 1 << p.lx_log2;
+  p.lanes_log2 = SHARED ? lanes_of_gate(p.width, VEC, p.lx_log2) : 0;
+  if (ctas > 2147483647LL) return TSB_ERR_TOO_LARGE;
+  const size_t bytes = S::bytes(lx, p.cluster);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(ctas * p.parts));
+  cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(kScanThreads + 32);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = stream;
@@ -650,7 +782,9 @@ inline int64_t partials_of_row(int64_t K, int64_t width, size_t elem) {
   int64_t most = 0;
   for (const int vec : {(int)(16 / elem), 2, 1}) {
     if (K % vec != 0 || width % vec != 0) continue;
-    const int64_t per = (int64_t)vec << lanes_of_gate(width, vec, lanes_of_row(K, vec, elem));
+    // (a launch may take fewer lanes for a row than there could be)
+    const int lanes = std::min(lanes_of_gate(width, vec, lanes_of_row(K, vec, elem)), least_lanes(vec));
+    const int64_t per = (int64_t)vec << lanes;
     if (per != width) most = std::max(most, K / per);
   }
   return most;
