@@ -6,6 +6,9 @@
 //
 // Both are bound by HBM: a pass moves T rows of few and T*k rows of many once.  Work is driven by the tokens, because a
 // row of few is then read (or written) once; driven by the places, dispatch would read it k times, far apart in time.
+// Rows move in 16-byte chunks.  Where the row length is no multiple of 16 bytes, chunks are those of the row that is
+// written, and the data comes out of the two aligned chunks of the source row that hold it, shifted into place: twice the
+// load instructions, but whole sectors and 16-byte stores instead of single values.
 #include <algorithm>
 
 #include "common.cuh"
@@ -23,90 +26,280 @@ struct RowsParams {
   int64_t T, k, K, M;
 };
 
-// one thread: one pack of one token
-template <typename T, int VEC, bool SPREAD>
+template <typename T> constexpr int chunk_len() { return 16 / (int)sizeof(T); }
+
+// elements [a, b) of a chunk belong to the row
+struct Span { int a, b; };
+
+// V elements from p on, wherever p is; those outside the span are 0.  lo, hi: the ends of the array p points into.
+template <typename T>
+__device__ __forceinline__ Pack<T, chunk_len<T>()> load_any(const T *p, Span s, const T *lo, const T *hi) {
+  constexpr int V = chunk_len<T>();
+  Pack<T, V> r;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p), base = at & ~(uintptr_t)15;
+  const int off = (int)(at & 15);
+  if (s.a == 0 && s.b == V && (off == 0 || (base >= reinterpret_cast<uintptr_t>(lo) && base + 32 <= reinterpret_cast<uintptr_t>(hi)))) {
+    const uint4 x = *reinterpret_cast<const uint4 *>(base);
+    if (off == 0) return *reinterpret_cast<const Pack<T, V> *>(&x);
+    const uint4 y = *reinterpret_cast<const uint4 *>(base + 16);
+    unsigned w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    if (off & 8) {
+#pragma unroll
+      for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (off & 4) {
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    if (off & 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+    }
+    return *reinterpret_cast<const Pack<T, V> *>(w);
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = i >= s.a && i < s.b ? p[i] : from_acc<T>((acc_t<T>)0);
+  return r;
+}
+template <typename T> __device__ __forceinline__ void store_span(T *p, const Pack<T, chunk_len<T>()> &v, Span s) {
+  constexpr int V = chunk_len<T>();
+  if (s.a == 0 && s.b == V) {
+    st_stream<T, V>(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i >= s.a && i < s.b) p[i] = v.v[i];
+  }
+}
+
+// The c-th 16-byte chunk of a row: its first element (negative where the row begins inside the chunk) and its span.
+template <typename T, bool ALIGNED> __device__ __forceinline__ int64_t chunk_of(const T *row, int64_t c, int64_t K, Span &s) {
+  constexpr int V = chunk_len<T>();
+  if constexpr (ALIGNED) {
+    s = {0, V};
+    return c * V;
+  } else {
+    const int64_t e0 = c * V - (int64_t)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    s.a = e0 < 0 ? (int)-e0 : 0;
+    s.b = K - e0 < V ? (int)(K - e0) : V;
+    return e0;
+  }
+}
+template <typename T, bool ALIGNED> __host__ __device__ __forceinline__ int64_t chunks_of(int64_t K) {
+  constexpr int V = chunk_len<T>();
+  return ALIGNED ? K / V : (K + 2 * V - 2) / V;
+}
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ Pack<T, chunk_len<T>()> load_chunk(const T *row, int64_t e0, Span s, const T *lo, const T *hi) {
+  if constexpr (ALIGNED) return ld_stream<T, chunk_len<T>()>(row + e0);
+  else return load_any<T>(row + e0, s, lo, hi);
+}
+template <typename T, typename A> __device__ __forceinline__ Pack<T, chunk_len<T>()> scaled(const Pack<T, chunk_len<T>()> &v, A w) {
+  Pack<T, chunk_len<T>()> o;
+#pragma unroll
+  for (int i = 0; i < chunk_len<T>(); ++i) o.v[i] = from_acc<T>(to_acc<T>(v.v[i]) * w);
+  return o;
+}
+
+// zeros for the rows of many that no token owns
+template <typename T, bool ALIGNED> __device__ __forceinline__ void zero_tail(const RowsParams &p, int64_t first, int64_t step) {
+  const int64_t used = clamp64(*p.used, 0, p.M);
+  T *tail = static_cast<T *>(p.many_out) + used * p.K;
+  constexpr int V = ALIGNED ? chunk_len<T>() : 1;
+  Pack<T, V> zero;
+#pragma unroll
+  for (int i = 0; i < V; ++i) zero.v[i] = from_acc<T>((acc_t<T>)0);
+  for (int64_t i = first; i < (p.M - used) * p.K / V; i += step) st_stream<T, V>(tail + i * V, zero);
+}
+
+// Without dot products: one thread, one chunk of one token.  The rows of several choices are in flight at once.
+template <typename T, bool SPREAD, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
   using A = acc_t<T>;
+  constexpr int V = chunk_len<T>(), J = 4;
   const A *__restrict__ weight = static_cast<const A *>(p.weight);
-  const int64_t Kv = p.K / VEC, items = p.T * Kv;
+  const T *few_in = static_cast<const T *>(p.few_in), *many_in = static_cast<const T *>(p.many_in);
+  T *few_out = static_cast<T *>(p.few_out), *many_out = static_cast<T *>(p.many_out);
+  const int64_t Kc = chunks_of<T, ALIGNED>(p.K), items = p.T * Kc;
   const int64_t step = (int64_t)gridDim.x * kThreads, first = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   for (int64_t it = first; it < items; it += step) {
-    const int64_t t = it / Kv, c = (it - t * Kv) * VEC;
+    const int64_t t = items <= 0xffffffffLL ? (int64_t)((unsigned)it / (unsigned)Kc) : it / Kc, c = it - t * Kc;
     const int64_t *slot = p.slot + t * p.k;
+    Span s;
     if constexpr (SPREAD) {
-      const Pack<T, VEC> v = ld_stream<T, VEC>(static_cast<const T *>(p.few_in) + t * p.K + c);
-      T *many = static_cast<T *>(p.many_out) + c;
+      Pack<T, V> v;
+      if constexpr (ALIGNED) v = ld_stream<T, V>(few_in + t * p.K + c * V);
       for (int64_t j = 0; j < p.k; ++j) {
         const int64_t to = slot[j];
         if (to < 0 || to >= p.M) continue;
-        Pack<T, VEC> o = v;
-        if (weight) {
-          const A w = weight[t * p.k + j];
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) o.v[i] = from_acc<T>(to_acc<T>(v.v[i]) * w);
+        T *row = many_out + to * p.K;
+        const int64_t e0 = chunk_of<T, ALIGNED>(row, c, p.K, s);
+        if constexpr (!ALIGNED) {
+          if (s.b <= s.a) continue;
+          v = load_any<T>(few_in + t * p.K + e0, s, few_in, few_in + p.T * p.K);
         }
-        st_stream<T, VEC>(many + to * p.K, o);
+        store_span<T>(row + e0, weight ? scaled<T, A>(v, weight[t * p.k + j]) : v, s);
       }
     } else {
-      const T *many = static_cast<const T *>(p.many_in) + c;
-      A sum[VEC];
+      T *row = few_out + t * p.K;
+      const int64_t e0 = chunk_of<T, ALIGNED>(row, c, p.K, s);
+      if (!ALIGNED && s.b <= s.a) continue;
+      A sum[V];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sum[i] = 0;
-      for (int64_t j = 0; j < p.k; ++j) {
-        const int64_t from = slot[j];
-        if (from < 0 || from >= p.M) continue;
-        const Pack<T, VEC> v = ld_stream<T, VEC>(many + from * p.K);
-        const A w = weight ? weight[t * p.k + j] : (A)1;
+      for (int i = 0; i < V; ++i) sum[i] = 0;
+      for (int64_t j0 = 0; j0 < p.k; j0 += J) {
+        Pack<T, V> v[J];
+        bool some[J];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sum[i] += to_acc<T>(v.v[i]) * w;
+        for (int j = 0; j < J; ++j) {
+          const int64_t from = j0 + j < p.k ? slot[j0 + j] : -1;
+          some[j] = from >= 0 && from < p.M;
+          if (some[j]) v[j] = load_chunk<T, ALIGNED>(many_in + from * p.K, e0, s, many_in, many_in + p.M * p.K);
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          if (!some[j]) continue;
+          const A w = weight ? weight[t * p.k + j0 + j] : (A)1;
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum[i] += to_acc<T>(v[j].v[i]) * w;
+        }
       }
-      Pack<T, VEC> o;
+      Pack<T, V> o;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) o.v[i] = from_acc<T>(sum[i]);
-      st_stream<T, VEC>(static_cast<T *>(p.few_out) + t * p.K + c, o);
+      for (int i = 0; i < V; ++i) o.v[i] = from_acc<T>(sum[i]);
+      store_span<T>(row + e0, o, s);
     }
   }
-  if constexpr (SPREAD) {
-    const int64_t used = clamp64(*p.used, 0, p.M);
-    T *tail = static_cast<T *>(p.many_out) + used * p.K;
-    Pack<T, VEC> zero;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) zero.v[i] = from_acc<T>((A)0);
-    for (int64_t it = first; it < (p.M - used) * Kv; it += step) st_stream<T, VEC>(tail + it * VEC, zero);
-  }
+  if constexpr (SPREAD) zero_tail<T, ALIGNED>(p, first, step);
 }
 
-// one warp: one (token, choice), its dot product
-template <typename T, int VEC>
+// With dot products: G threads (lanes of a warp, or the CTA) walk one token's chunks, J choices at a time.  WRITE: also
+// spread or fold; a fold needs all choices of a chunk at once, so it has J >= k.
+template <typename T, bool SPREAD, bool ALIGNED, bool WRITE, int J, int G>
 __global__ void __launch_bounds__(kThreads) rows_dot_kernel(RowsParams p) {
   using A = acc_t<T>;
-  const int lane = threadIdx.x & 31;
-  const int64_t step = (int64_t)gridDim.x * (kThreads / 32);
-  for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < p.M; i += step) {
-    const int64_t t = i / p.k, at = p.slot[i];
-    A sum = 0;
-    if (at >= 0 && at < p.M) {
-      const T *a = static_cast<const T *>(p.few_in) + t * p.K, *b = static_cast<const T *>(p.many_in) + at * p.K;
-      for (int64_t c = (int64_t)lane * VEC; c < p.K; c += 32 * VEC) {
-        const Pack<T, VEC> x = ld_pack<T, VEC>(a + c), y = ld_stream<T, VEC>(b + c);
+  constexpr int V = chunk_len<T>(), kGroups = kThreads / G, kWarps = kThreads / 32;
+  __shared__ A s_part[G > 32 ? kWarps * J : 1];
+  const A *__restrict__ weight = static_cast<const A *>(p.weight);
+  const T *few_in = static_cast<const T *>(p.few_in), *many_in = static_cast<const T *>(p.many_in);
+  T *few_out = static_cast<T *>(p.few_out), *many_out = static_cast<T *>(p.many_out);
+  A *dot = static_cast<A *>(p.dot);
+  const int64_t Kc = chunks_of<T, ALIGNED>(p.K);
+  const int lane = threadIdx.x % G, group = threadIdx.x / G;
+  // whole warps stay together: the last round of tokens may hold groups without one
+  for (int64_t t0 = (int64_t)blockIdx.x * kGroups; t0 < p.T; t0 += (int64_t)gridDim.x * kGroups) {
+    const int64_t t = t0 + group;
+    const bool live = t < p.T;
+    for (int64_t j0 = 0; j0 < p.k; j0 += J) {
+      int64_t at[J];
+      A w[J], sum[J];
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) sum += to_acc<T>(x.v[q]) * to_acc<T>(y.v[q]);
+      for (int j = 0; j < J; ++j) {
+        const int64_t i = live && j0 + j < p.k ? p.slot[t * p.k + j0 + j] : -1;
+        at[j] = i < p.M ? i : -1;
+        w[j] = weight && at[j] >= 0 ? weight[t * p.k + j0 + j] : (A)1;
+        sum[j] = 0;
+      }
+      if (live) {
+        const T *few = few_in + t * p.K;
+        for (int64_t c = lane; c < Kc; c += G) {
+          Pack<T, V> x, y[J];
+          Span s;
+          int64_t e0 = 0;
+          if constexpr (ALIGNED || !SPREAD) {
+            e0 = chunk_of<T, ALIGNED>(SPREAD || !WRITE ? few : few_out + t * p.K, c, p.K, s);
+            if (!ALIGNED && s.b <= s.a) continue;
+            x = load_chunk<T, ALIGNED>(few, e0, s, few_in, few_in + p.T * p.K);
+          }
+          A fold[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) fold[i] = 0;
+          if constexpr (ALIGNED || !SPREAD) {
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+              if (at[j] >= 0) y[j] = load_chunk<T, ALIGNED>(many_in + at[j] * p.K, e0, s, many_in, many_in + p.M * p.K);
+          }
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            if (at[j] < 0) continue;
+            if constexpr (!ALIGNED && SPREAD) {  // the chunks of this choice's row
+              e0 = chunk_of<T, false>(many_out + at[j] * p.K, c, p.K, s);
+              if (s.b <= s.a) continue;
+              x = load_any<T>(few + e0, s, few_in, few_in + p.T * p.K);
+              y[j] = load_any<T>(many_in + at[j] * p.K + e0, s, many_in, many_in + p.M * p.K);
+            }
+            if constexpr (SPREAD && WRITE) store_span<T>(many_out + at[j] * p.K + e0, weight ? scaled<T, A>(x, w[j]) : x, s);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const A a = to_acc<T>(y[j].v[i]);
+              sum[j] += to_acc<T>(x.v[i]) * a;
+              if (!SPREAD && WRITE) fold[i] += a * w[j];
+            }
+          }
+          if constexpr (!SPREAD && WRITE) {
+            Pack<T, V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = from_acc<T>(fold[i]);
+            store_span<T>(few_out + t * p.K + e0, o, s);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+#pragma unroll
+        for (int m = (G < 32 ? G : 32) / 2; m; m >>= 1) sum[j] += shfl_xor(sum[j], m);
+      }
+      if constexpr (G > 32) {
+        if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+          for (int j = 0; j < J; ++j) s_part[(threadIdx.x >> 5) * J + j] = sum[j];
+        }
+        __syncthreads();
+        if (threadIdx.x < J && j0 + threadIdx.x < p.k) {
+          A all = 0;
+          for (int i = 0; i < kWarps; ++i) all += s_part[i * J + threadIdx.x];
+          dot[t * p.k + j0 + threadIdx.x] = all;
+        }
+        __syncthreads();
+      } else if (live) {
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if (lane == j % G && j0 + j < p.k) dot[t * p.k + j0 + j] = sum[j];
       }
     }
-#pragma unroll
-    for (int m = 16; m; m >>= 1) sum += shfl_xor(sum, m);
-    if (lane == 0) static_cast<A *>(p.dot)[i] = sum;
   }
+  if constexpr (SPREAD && WRITE) zero_tail<T, ALIGNED>(p, (int64_t)blockIdx.x * kThreads + threadIdx.x, (int64_t)gridDim.x * kThreads);
 }
 
-template <typename T, int VEC, bool SPREAD> int launch_rows(const RowsParams &p, cudaStream_t stream) {
-  const int64_t most = (int64_t)sm_count() * 64;
-  const int64_t blocks = std::max<int64_t>(1, std::min(most, (p.T * (p.K / VEC) + kThreads - 1) / kThreads));
-  rows_kernel<T, VEC, SPREAD><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
-  if (p.dot) {
-    const int64_t warps = std::min(most, (p.M + kThreads / 32 - 1) / (kThreads / 32));
-    rows_dot_kernel<T, VEC><<<(unsigned)warps, kThreads, 0, stream>>>(p);
-  }
+template <typename T, bool SPREAD, bool ALIGNED, bool WRITE> int launch_dot(const RowsParams &p, cudaStream_t stream) {
+  const auto go = [&](auto jn, auto gn) {
+    constexpr int J = decltype(jn)::value, G = decltype(gn)::value;
+    const int64_t want = (p.T + kThreads / G - 1) / (kThreads / G);
+    const int64_t blocks = std::min<int64_t>(want, (int64_t)sm_count() * 32);
+    rows_dot_kernel<T, SPREAD, ALIGNED, WRITE, J, G><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
+    return launch_status();
+  };
+  const auto with_j = [&](auto gn) {
+    if constexpr (WRITE) {  // (the products alone are only asked for where there are more than eight choices)
+      if (p.k <= 2) return go(std::integral_constant<int, 2>(), gn);
+      if (p.k <= 4) return go(std::integral_constant<int, 4>(), gn);
+    }
+    return go(std::integral_constant<int, 8>(), gn);
+  };
+  // Threads of a token: what its chunks keep busy, and a whole CTA where the tokens alone would not fill the GPU.
+  const int64_t Kc = chunks_of<T, ALIGNED>(p.K);
+  if (Kc <= 8) return with_j(std::integral_constant<int, 8>());
+  if (Kc <= 32 || p.T >= (int64_t)sm_count() * 16) return with_j(std::integral_constant<int, 32>());
+  return with_j(std::integral_constant<int, kThreads>());
+}
+
+template <typename T, bool SPREAD, bool ALIGNED> int launch_rows(const RowsParams &p, cudaStream_t stream) {
+  if (p.dot && (SPREAD || p.k <= 8)) return launch_dot<T, SPREAD, ALIGNED, true>(p, stream);
+  const int64_t items = p.T * chunks_of<T, ALIGNED>(p.K);
+  const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((int64_t)sm_count() * 64, (items + kThreads - 1) / kThreads));
+  rows_kernel<T, SPREAD, ALIGNED><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
+  if constexpr (!SPREAD)
+    if (p.dot) return launch_dot<T, SPREAD, ALIGNED, false>(p, stream);
   return launch_status();
 }
 
@@ -119,8 +312,7 @@ template <bool SPREAD> int rows_entry(const RowsParams &p, int dtype, cudaStream
   const bool aligned = aligned16(p.few_in) && aligned16(p.many_in) && aligned16(p.few_out) && aligned16(p.many_out);
   const auto go = [&](auto type) {
     using T = decltype(type);
-    constexpr int full = full_vec<T>();
-    return aligned && p.K % full == 0 ? launch_rows<T, full, SPREAD>(p, stream) : launch_rows<T, 1, SPREAD>(p, stream);
+    return aligned && p.K % chunk_len<T>() == 0 ? launch_rows<T, SPREAD, true>(p, stream) : launch_rows<T, SPREAD, false>(p, stream);
   };
   switch (dtype) {
     case TSB_F32: return go(float());

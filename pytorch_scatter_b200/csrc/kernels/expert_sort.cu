@@ -1,98 +1,181 @@
 // Tokens sorted by expert: a stable counting sort of n entries over E experts.
 //
-// Every block owns a contiguous chunk of entries, every warp of it a contiguous part of the chunk.  (1) each block counts
-// its entries per expert; (2) one block turns the counts, expert by expert and block by block inside an expert, into the
-// first place of each (expert, block); (3) each block counts again per warp and hands out places in entry order, the
-// rank inside 32 entries coming from a match of the expert ids.  Nothing depends on the order in which blocks run.
+// Every block owns a contiguous range of entries, every warp of it a contiguous part of that.  (1) Each block counts its
+// entries per expert.  (2) Each block adds up the counts of all blocks, which gives the first place of every expert and
+// its own first place inside it, counts again per warp, and hands out places in entry order, the rank inside 32 entries
+// coming from a match of the expert ids.  Up to kOneBlock entries one block does without (1).  Nothing depends on the
+// order in which blocks run, and no float is involved.
+//
+// Bound by the 24 bytes of each entry that are read and written, and below some 100,000 entries by the two launches and
+// the latency of the counts.
+#include <algorithm>
+#include <atomic>
+
 #include "common.cuh"
 
 namespace tsb {
 namespace {
 
-constexpr int kSortWarps = 8;
-constexpr int kSortPerWarp = 512;                         // entries of a warp
-constexpr int kSortChunk = kSortWarps * kSortPerWarp;     // entries of a block
+constexpr int kSortThreads = 1024;
+constexpr int64_t kOneBlock = 8192;          // entries
 constexpr int64_t kSortMostExperts = 4096;
+constexpr int kCountInts = 48 * 1024;        // shared memory for the counts of the warps
+constexpr int kBatch = 8;                    // index loads in flight of a warp, 32 entries each
 
 // experts 0 .. E-1, and one more bucket E for entries that name none
 __device__ __forceinline__ int bucket_of(int64_t e, int E) { return e >= 0 && e < E ? (int)e : E; }
 
-__global__ void __launch_bounds__(kSortWarps * 32) sort_count_kernel(const int64_t *__restrict__ index, int *__restrict__ counts,
-                                                                     int64_t n, int E, int blocks) {
+// The entries of a warp, 32 at a time and in order: f(first entry of the 32, bucket of this lane's, -1 behind the end)
+template <typename F> __device__ __forceinline__ void each_entry(const int64_t *__restrict__ index, int64_t lo, int64_t hi, int E, F f) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t i0 = lo; i0 < hi; i0 += 32 * kBatch) {
+    int64_t e[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int64_t i = i0 + b * 32 + lane;
+      e[b] = i < hi ? index[i] : 0;
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int64_t i = i0 + b * 32;
+      if (i >= hi) break;
+      f(i, i + lane < hi ? bucket_of(e[b], E) : -1);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kSortThreads)
+sort_count_kernel(const int64_t *__restrict__ index, int *__restrict__ counts, int64_t n, int E, int64_t per_block) {
   extern __shared__ int s_count[];
   for (int e = threadIdx.x; e <= E; e += blockDim.x) s_count[e] = 0;
   __syncthreads();
-  const int64_t lo = (int64_t)blockIdx.x * kSortChunk;
-  for (int i = threadIdx.x; i < kSortChunk; i += blockDim.x)
-    if (lo + i < n) atomicAdd(&s_count[bucket_of(index[lo + i], E)], 1);
+  const int64_t lo = min(blockIdx.x * per_block, n), hi = min(lo + per_block, n);
+  const int64_t part = (hi - lo + blockDim.x / 32 - 1) / (blockDim.x / 32), wlo = lo + (threadIdx.x >> 5) * part;
+  each_entry(index, min(wlo, hi), min(wlo + part, hi), E, [&](int64_t, int e) {
+    if (e >= 0) atomicAdd(&s_count[e], 1);
+  });
   __syncthreads();
-  for (int e = threadIdx.x; e <= E; e += blockDim.x) counts[(int64_t)e * blocks + blockIdx.x] = s_count[e];
+  for (int e = threadIdx.x; e <= E; e += blockDim.x) counts[(int64_t)blockIdx.x * (E + 1) + e] = s_count[e];
 }
 
-// counts [E+1][blocks] -> exclusive prefix sums in place; indptr
-__global__ void __launch_bounds__(1024) sort_prefix_kernel(int *__restrict__ counts, int64_t *__restrict__ indptr, int E, int blocks) {
-  __shared__ int s_warp[32];
-  const int64_t total = (int64_t)(E + 1) * blocks;
-  const int64_t per = (total + 1023) / 1024;
-  const int64_t lo = min((int64_t)threadIdx.x * per, total), hi = min(lo + per, total);
-  int sum = 0;
-  for (int64_t i = lo; i < hi; ++i) sum += counts[i];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int incl = sum;
-  for (int d = 1; d < 32; d <<= 1) {
-    const int v = __shfl_up_sync(kFullMask, incl, d);
-    if (lane >= d) incl += v;
-  }
-  if (lane == 31) s_warp[warp] = incl;
+// shared: [E+1] first places, [warps][E+1] counts of the warps, later their next places
+__global__ void __launch_bounds__(kSortThreads)
+sort_place_kernel(const int64_t *__restrict__ index, const int *__restrict__ counts, int64_t *__restrict__ slot,
+                  int64_t *__restrict__ order, int64_t *__restrict__ indptr, int64_t n, int E, int64_t per_block, int warps) {
+  extern __shared__ int s_all[];
+  __shared__ int s_sum[32];
+  int *s_first = s_all, *s_warp = s_all + (E + 1);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, blocks = gridDim.x;
+  // the first `warps` warps carry entries; the experts are spread over all threads
+  int *mine = s_warp + warp * (E + 1);
+  for (int i = threadIdx.x; i < warps * (E + 1); i += blockDim.x) s_warp[i] = 0;
   __syncthreads();
-  int run = incl - sum;
-  for (int w = 0; w < warp; ++w) run += s_warp[w];
-  for (int64_t i = lo; i < hi; ++i) {
-    const int c = counts[i];
-    counts[i] = run;
-    if (i % blocks == 0) indptr[i / blocks] = run;
-    run += c;
-  }
-}
+  const int64_t lo = min(blockIdx.x * per_block, n), hi = min(lo + per_block, n);
+  const int64_t part = (hi - lo + warps - 1) / warps, wlo = warp < warps ? min(lo + warp * part, hi) : hi, whi = min(wlo + part, hi);
+  each_entry(index, wlo, whi, E, [&](int64_t, int e) {
+    if (e >= 0) atomicAdd(&mine[e], 1);
+  });
 
-__global__ void __launch_bounds__(kSortWarps * 32)
-sort_place_kernel(const int64_t *__restrict__ index, const int *__restrict__ first, int64_t *__restrict__ slot,
-                  int64_t *__restrict__ order, int64_t n, int E, int blocks) {
-  extern __shared__ int s_place[];  // [warps][E+1]
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int e = threadIdx.x; e < kSortWarps * (E + 1); e += blockDim.x) s_place[e] = 0;
-  __syncthreads();
-  const int64_t lo = (int64_t)blockIdx.x * kSortChunk + warp * kSortPerWarp;
-  int *mine = s_place + warp * (E + 1);
-  for (int i = lane; i < kSortPerWarp; i += 32)
-    if (lo + i < n) atomicAdd(&mine[bucket_of(index[lo + i], E)], 1);
-  __syncthreads();
-  for (int e = threadIdx.x; e <= E; e += blockDim.x) {
-    int run = first[(int64_t)e * blocks + blockIdx.x];
-    for (int w = 0; w < kSortWarps; ++w) {
-      const int c = s_place[w * (E + 1) + e];
-      s_place[w * (E + 1) + e] = run;
-      run += c;
+  // entries of each expert before this block and in all blocks
+  constexpr int kMine = (kSortMostExperts + kSortThreads) / kSortThreads;  // experts of a thread
+  int before[kMine] = {}, total[kMine] = {};
+  if (counts) {
+    // several threads share an expert's column where there are more threads than experts
+    const int groups = max(1, (int)blockDim.x / (E + 1));
+    if (groups > 1) {
+      int *s_part = s_first;  // [E+1] x (before, all) by atomics: integers, any order gives the same sums
+      __shared__ int s_before[kSortThreads];
+      for (int e = threadIdx.x; e <= E; e += blockDim.x) s_part[e] = s_before[e] = 0;
+      __syncthreads();
+      const int e = threadIdx.x % (E + 1), g = threadIdx.x / (E + 1);
+      if (g < groups) {
+        int all = 0, bef = 0;
+#pragma unroll 8
+        for (int b = g; b < blocks; b += groups) {
+          const int c = counts[(int64_t)b * (E + 1) + e];
+          all += c;
+          bef += b < (int)blockIdx.x ? c : 0;
+        }
+        atomicAdd(&s_part[e], all);
+        atomicAdd(&s_before[e], bef);
+      }
+      __syncthreads();
+      if (threadIdx.x <= E) {
+        total[0] = s_part[threadIdx.x];
+        before[0] = s_before[threadIdx.x];
+      }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int q = 0; q < kMine; ++q) {
+        const int e = q * blockDim.x + threadIdx.x;
+        if (e > E) break;
+#pragma unroll 8
+        for (int b = 0; b < blocks; ++b) {
+          const int c = counts[(int64_t)b * (E + 1) + e];
+          total[q] += c;
+          before[q] += b < (int)blockIdx.x ? c : 0;
+        }
+      }
+    }
+    __syncthreads();
+  } else {
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kMine; ++q) {
+      const int e = q * blockDim.x + threadIdx.x;
+      if (e > E) break;
+      for (int w = 0; w < warps; ++w) total[q] += s_warp[w * (E + 1) + e];
     }
   }
-  __syncthreads();
-  for (int i = lane; i < kSortPerWarp; i += 32) {
-    const bool in = lo + i < n;
-    const unsigned active = __ballot_sync(kFullMask, in);
-    if (in) {
-      const int e = bucket_of(index[lo + i], E);
-      const unsigned peers = __match_any_sync(active, e);
-      const int place = mine[e] + __popc(peers & ((1u << lane) - 1u));
-      __syncwarp(active);
+
+  // first place of each expert: prefix sums of the totals, a row of threads after the other
+  int run = 0;
+#pragma unroll
+  for (int q = 0; q < kMine; ++q) {
+    if (q * (int)blockDim.x > E) break;
+    int incl = total[q];
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(kFullMask, incl, d);
+      if (lane >= d) incl += v;
+    }
+    if (lane == 31) s_sum[warp] = incl;
+    __syncthreads();
+    int add = run;
+    for (int w = 0; w < (int)blockDim.x >> 5; ++w) {
+      if (w < warp) add += s_sum[w];
+      run += s_sum[w];
+    }
+    const int e = q * blockDim.x + threadIdx.x;
+    if (e <= E) {
+      int place = add + incl - total[q];
+      if (blockIdx.x == 0) indptr[e] = place;
+      place += before[q];
+      for (int w = 0; w < warps; ++w) {
+        const int c = s_warp[w * (E + 1) + e];
+        s_warp[w * (E + 1) + e] = place;
+        place += c;
+      }
+    }
+    __syncthreads();
+  }
+
+  each_entry(index, wlo, whi, E, [&](int64_t i, int e) {
+    const unsigned peers = __match_any_sync(kFullMask, e);
+    int place = 0;
+    if (e >= 0) place = mine[e] + __popc(peers & ((1u << lane) - 1u));
+    __syncwarp();
+    if (e >= 0) {
       if ((peers >> lane) == 1u) mine[e] = place + 1;  // the last of the peers
-      slot[lo + i] = e < E ? place : -1;
-      order[place] = lo + i;
+      slot[i + lane] = e < E ? place : -1;
+      order[place] = i + lane;
     }
     __syncwarp();
-  }
+  });
 }
 
-int64_t sort_blocks(int64_t n) { return (n + kSortChunk - 1) / kSortChunk; }
+// blocks and the entries of each: one block for few entries, else a multiple of what keeps every SM busy
+int64_t sort_blocks(int64_t n) { return n <= kOneBlock ? 1 : std::min<int64_t>(148, (n + 2047) / 2048); }
 
 }  // namespace
 }  // namespace tsb
@@ -100,7 +183,7 @@ int64_t sort_blocks(int64_t n) { return (n + kSortChunk - 1) / kSortChunk; }
 using namespace tsb;
 
 extern "C" size_t tsb_expert_sort_workspace_bytes(int64_t n, int64_t E) {
-  if (n < 0 || E < 0) return 0;
+  if (n < 0 || E < 0 || n <= kOneBlock) return 0;
   const size_t bytes = sizeof(int) * (size_t)(E + 1) * (size_t)sort_blocks(n);
   return (bytes + 255) / 256 * 256;
 }
@@ -112,15 +195,22 @@ extern "C" int tsb_expert_sort(const int64_t *index, int64_t *slot, int64_t *ord
   cudaStream_t st = (cudaStream_t)stream;
   if (n == 0) return cudaMemsetAsync(indptr, 0, sizeof(int64_t) * (E + 1), st) == cudaSuccess ? TSB_OK : TSB_ERR_LAUNCH;
   if (!index || !slot || !order) return TSB_ERR_ARG;
-  if (!workspace || workspace_bytes < tsb_expert_sort_workspace_bytes(n, E)) return TSB_ERR_WORKSPACE;
-  const int blocks = (int)sort_blocks(n);
-  int *counts = static_cast<int *>(workspace);
-  const size_t one = sizeof(int) * (E + 1), all = one * kSortWarps;
-  if (all > 48 * 1024 &&
-      cudaFuncSetAttribute(sort_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)all) != cudaSuccess)
-    return TSB_ERR_LAUNCH;
-  sort_count_kernel<<<blocks, kSortWarps * 32, one, st>>>(index, counts, n, (int)E, blocks);
-  sort_prefix_kernel<<<1, 1024, 0, st>>>(counts, indptr, (int)E, blocks);
-  sort_place_kernel<<<blocks, kSortWarps * 32, all, st>>>(index, counts, slot, order, n, (int)E, blocks);
+  if (n > kOneBlock && (!workspace || workspace_bytes < tsb_expert_sort_workspace_bytes(n, E))) return TSB_ERR_WORKSPACE;
+  static std::atomic<bool> allowed[64];  // per device; setting the attribute twice is harmless
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TSB_ERR_LAUNCH;
+  if (!allowed[dev]) {
+    if (cudaFuncSetAttribute(sort_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kCountInts + (int)kSortMostExperts + 1) * (int)sizeof(int)) != cudaSuccess)
+      return TSB_ERR_LAUNCH;
+    allowed[dev] = true;
+  }
+  const int64_t blocks = sort_blocks(n), per_block = (n + blocks - 1) / blocks;
+  // warps: one for each 32 entries, as many as their counts leave room for (11 with 4096 experts)
+  const int64_t warps = std::max<int64_t>(1, std::min<int64_t>({32, (per_block + 31) / 32, (int64_t)kCountInts / (E + 1)}));
+  int *counts = blocks > 1 ? static_cast<int *>(workspace) : nullptr;
+  const size_t one = sizeof(int) * (E + 1);
+  if (counts) sort_count_kernel<<<(unsigned)blocks, kSortThreads, one, st>>>(index, counts, n, (int)E, per_block);
+  const int64_t threads = std::max<int64_t>(warps * 32, std::min<int64_t>(kSortThreads, (E + 32) / 32 * 32));
+  sort_place_kernel<<<(unsigned)blocks, (unsigned)threads, one * (warps + 1), st>>>(index, counts, slot, order, indptr, n, (int)E, per_block, (int)warps);
   return launch_status();
 }
