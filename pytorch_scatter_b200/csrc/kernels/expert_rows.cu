@@ -10,8 +10,9 @@
 // written, and the data comes out of the two aligned chunks of the source row that hold it, shifted into place: twice the
 // load instructions, but whole sectors and 16-byte stores instead of single values.
 #include <algorithm>
+#include <atomic>
 
-#include "common.cuh"
+#include "mbarrier.cuh"
 
 namespace tsb {
 namespace {
@@ -113,10 +114,10 @@ template <typename T, bool ALIGNED> __device__ __forceinline__ void zero_tail(co
 }
 
 // Without dot products: one thread, one chunk of one token.  The rows of several choices are in flight at once.
-template <typename T, bool SPREAD, bool ALIGNED>
+template <typename T, bool SPREAD, bool ALIGNED, int J>
 __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
   using A = acc_t<T>;
-  constexpr int V = chunk_len<T>(), J = 4;
+  constexpr int V = chunk_len<T>();
   const A *__restrict__ weight = static_cast<const A *>(p.weight);
   const T *few_in = static_cast<const T *>(p.few_in), *many_in = static_cast<const T *>(p.many_in);
   T *few_out = static_cast<T *>(p.few_out), *many_out = static_cast<T *>(p.many_out);
@@ -271,6 +272,179 @@ __global__ void __launch_bounds__(kThreads) rows_dot_kernel(RowsParams p) {
   if constexpr (SPREAD && WRITE) zero_tail<T, ALIGNED>(p, (int64_t)blockIdx.x * kThreads + threadIdx.x, (int64_t)gridDim.x * kThreads);
 }
 
+// Long aligned rows of many tokens.  Every warp runs a pipeline of its own: bulk copies bring pieces of its tokens' rows
+// into a ring in shared memory, several steps ahead of the step that is summed, scaled or stored, so the bytes in flight
+// depend neither on registers nor on occupancy.  Lane j carries the j-th choice.  An unweighted spread only passes
+// through: bulk stores take the piece to its k places.
+constexpr int kBulkWarps = 8, kBulkMostStages = 8, kBulkWarpBytes = 12 * 1024, kBulkChunks = 4;
+constexpr int kBulkSmem = kBulkWarps * kBulkWarpBytes;
+
+struct BulkShape { int piece, stages, rows; };  // bytes of a row in a step, steps in the ring, rows of a step
+
+template <typename T, bool SPREAD, bool DOT>
+__global__ void __launch_bounds__(kBulkWarps * 32, 2) rows_bulk_kernel(RowsParams p, BulkShape shape) {
+  using A = acc_t<T>;
+  constexpr int V = chunk_len<T>(), U = kBulkChunks;
+  constexpr bool kFew = SPREAD || DOT, kMany = !SPREAD || DOT;
+  extern __shared__ __align__(128) char s_ring[];
+  __shared__ __align__(8) uint64_t s_bar[kBulkWarps][kBulkMostStages];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = (int)p.k;
+  const unsigned ring = smem_at(s_ring) + warp * kBulkWarpBytes, bar = smem_at(&s_bar[warp][0]);
+  const char *ring_p = s_ring + warp * kBulkWarpBytes;
+  if (lane < shape.stages) mbar_init(bar + lane * 8);
+  mbar_init_done();
+  __syncwarp();
+
+  const A *weight = static_cast<const A *>(p.weight);
+  const int64_t row_bytes = p.K * (int64_t)sizeof(T);
+  const int pieces = (int)((row_bytes + shape.piece - 1) / shape.piece), step_bytes = shape.rows * shape.piece;
+  const int64_t warps = (int64_t)gridDim.x * kBulkWarps, first = (int64_t)blockIdx.x * kBulkWarps + warp;
+  const char *few_in = static_cast<const char *>(p.few_in), *many_in = static_cast<const char *>(p.many_in);
+  char *few_out = static_cast<char *>(p.few_out), *many_out = static_cast<char *>(p.many_out);
+  const auto slot_of = [&](int64_t t) -> int64_t {
+    if (t >= p.T || lane >= k) return -1;
+    const int64_t s = p.slot[t * k + lane];
+    return s < p.M ? s : -1;
+  };
+
+  // the step that is issued next, its token's slots, and the slots of the token behind it
+  int64_t it = first, islot = slot_of(first), inext = slot_of(first + warps);
+  int ipiece = 0, istage = 0;
+  const auto issue = [&]() {
+    if (it < p.T) {
+      const int64_t off = (int64_t)ipiece * shape.piece;
+      const unsigned len = (unsigned)(row_bytes - off < shape.piece ? row_bytes - off : shape.piece);
+      const unsigned b = bar + istage * 8, to = ring + istage * step_bytes;
+      const bool mine = kMany && islot >= 0;
+      const int rows = __popc(__ballot_sync(kFullMask, mine)) + (kFew ? 1 : 0);
+      if (lane == 0) mbar_expect(b, rows * len);
+      __syncwarp();
+      if (kFew && lane == 0) bulk_load(to, few_in + it * row_bytes + off, len, b);
+      if (mine) bulk_load(to + (lane + (kFew ? 1 : 0)) * shape.piece, many_in + islot * row_bytes + off, len, b);
+      if (++ipiece == pieces) {
+        ipiece = 0;
+        it += warps;
+        islot = inext;
+        inext = slot_of(it + warps);
+      }
+    }
+    istage = istage + 1 == shape.stages ? 0 : istage + 1;
+  };
+  for (int i = 0; i < shape.stages - 1; ++i) issue();
+
+  int stage = 0;
+  unsigned phase = 0;
+  for (int64_t t = first; t < p.T; t += warps) {
+    const int64_t my_slot = slot_of(t);
+    const A my_weight = weight && lane < k ? weight[t * k + lane] : (A)1;
+    const unsigned valid = __ballot_sync(kFullMask, my_slot >= 0);
+    A my_dot = 0;
+    for (int q = 0; q < pieces; ++q) {
+      const int64_t off = (int64_t)q * shape.piece;
+      const int len = (int)(row_bytes - off < shape.piece ? row_bytes - off : shape.piece);
+      const bool came = mbar_wait(bar + stage * 8, phase);
+      const char *at = ring_p + stage * step_bytes;
+      if constexpr (SPREAD && !DOT) {
+        if (!weight) {
+          if (my_slot >= 0 && came) bulk_store(many_out + my_slot * row_bytes + off, ring + stage * step_bytes, len);
+          bulk_commit();
+          bulk_read_done<1>();  // the step before has left its place in the ring, which issue() fills again
+          __syncwarp();
+          issue();
+          if (++stage == shape.stages) { stage = 0; phase ^= 1; }
+          continue;
+        }
+      }
+      for (int c0 = lane * 16; c0 - lane * 16 < len; c0 += 32 * 16 * U) {
+        Pack<T, V> few[U];
+        A sum[U][V];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int c = c0 + u * 512;
+          if (kFew && c < len) few[u] = *reinterpret_cast<const Pack<T, V> *>(at + c);
+          if (SPREAD && !came) few[u] = scaled<T, A>(few[u], (A)NAN);
+          if constexpr (!SPREAD) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[u][i] = came ? (A)0 : (A)NAN;
+          }
+        }
+        for (int j = 0; j < k; ++j) {
+          if (!(valid >> j & 1)) continue;
+          const A w = __shfl_sync(kFullMask, my_weight, j);
+          A d = 0;
+          const char *row = at + (j + (kFew ? 1 : 0)) * shape.piece;
+          const int64_t to = SPREAD ? __shfl_sync(kFullMask, my_slot, j) * row_bytes + off : 0;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int c = c0 + u * 512;
+            if (c >= len) continue;
+            Pack<T, V> m;
+            if constexpr (kMany) m = *reinterpret_cast<const Pack<T, V> *>(row + c);
+            if constexpr (DOT) {
+#pragma unroll
+              for (int i = 0; i < V; ++i) d += to_acc<T>(few[u].v[i]) * to_acc<T>(m.v[i]);
+            }
+            if constexpr (SPREAD) {
+              st_stream<T, V>(reinterpret_cast<T *>(many_out + to + c), weight ? scaled<T, A>(few[u], w) : few[u]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < V; ++i) sum[u][i] += to_acc<T>(m.v[i]) * w;
+            }
+          }
+          if constexpr (DOT) {
+#pragma unroll
+            for (int s = 16; s; s >>= 1) d += shfl_xor(d, s);
+            if (lane == j) my_dot += came ? d : (A)NAN;
+          }
+        }
+        if constexpr (!SPREAD) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int c = c0 + u * 512;
+            if (c >= len) continue;
+            Pack<T, V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = from_acc<T>(sum[u][i]);
+            st_stream<T, V>(reinterpret_cast<T *>(few_out + t * row_bytes + off + c), o);
+          }
+        }
+      }
+      __syncwarp();  // all lanes have read the step: its place may be filled again
+      issue();
+      if (++stage == shape.stages) { stage = 0; phase ^= 1; }
+    }
+    if (DOT && lane < k) static_cast<A *>(p.dot)[t * k + lane] = my_dot;
+  }
+  if constexpr (SPREAD) {
+    zero_tail<T, true>(p, (int64_t)blockIdx.x * kBulkWarps * 32 + threadIdx.x, (int64_t)gridDim.x * kBulkWarps * 32);
+    bulk_read_done<0>();
+  }
+}
+
+// Whether the pipeline takes the problem: enough tokens for every warp to have some, rows of 512 bytes and more, and at
+// least three steps in the ring.
+template <typename T, bool SPREAD, bool DOT> bool bulk_shape(const RowsParams &p, BulkShape &s) {
+  const int64_t row_bytes = p.K * (int64_t)sizeof(T);
+  if (p.k > 32 || row_bytes < 512 || row_bytes > 1 << 30 || p.T < (int64_t)sm_count() * kBulkWarps * 2) return false;
+  s.rows = (SPREAD || DOT ? 1 : 0) + (!SPREAD || DOT ? (int)p.k : 0);
+  s.piece = 4096;
+  while (s.piece > 512 && (s.piece > row_bytes || s.rows * s.piece * 4 > kBulkWarpBytes)) s.piece /= 2;
+  s.stages = std::min(kBulkMostStages, kBulkWarpBytes / (s.rows * s.piece));
+  return s.stages >= 3;
+}
+
+template <typename T, bool SPREAD, bool DOT> int launch_bulk(const RowsParams &p, const BulkShape &shape, cudaStream_t stream) {
+  static std::atomic<bool> allowed[64];  // per device; setting the attribute twice is harmless
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TSB_ERR_LAUNCH;
+  if (!allowed[dev]) {
+    if (cudaFuncSetAttribute(rows_bulk_kernel<T, SPREAD, DOT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBulkSmem) != cudaSuccess) return TSB_ERR_LAUNCH;
+    allowed[dev] = true;
+  }
+  rows_bulk_kernel<T, SPREAD, DOT><<<(unsigned)sm_count() * 2, kBulkWarps * 32, kBulkSmem, stream>>>(p, shape);
+  return launch_status();
+}
+
 template <typename T, bool SPREAD, bool ALIGNED, bool WRITE> int launch_dot(const RowsParams &p, cudaStream_t stream) {
   const auto go = [&](auto jn, auto gn) {
     constexpr int J = decltype(jn)::value, G = decltype(gn)::value;
@@ -294,10 +468,20 @@ template <typename T, bool SPREAD, bool ALIGNED, bool WRITE> int launch_dot(cons
 }
 
 template <typename T, bool SPREAD, bool ALIGNED> int launch_rows(const RowsParams &p, cudaStream_t stream) {
+  if constexpr (ALIGNED) {
+    BulkShape shape;
+    if (p.dot ? bulk_shape<T, SPREAD, true>(p, shape) : bulk_shape<T, SPREAD, false>(p, shape))
+      return p.dot ? launch_bulk<T, SPREAD, true>(p, shape, stream) : launch_bulk<T, SPREAD, false>(p, shape, stream);
+  }
   if (p.dot && (SPREAD || p.k <= 8)) return launch_dot<T, SPREAD, ALIGNED, true>(p, stream);
   const int64_t items = p.T * chunks_of<T, ALIGNED>(p.K);
   const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((int64_t)sm_count() * 64, (items + kThreads - 1) / kThreads));
-  rows_kernel<T, SPREAD, ALIGNED><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
+  if constexpr (SPREAD) {
+    rows_kernel<T, true, ALIGNED, 1><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
+  } else {
+    if (p.k <= 2) rows_kernel<T, false, ALIGNED, 2><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
+    else rows_kernel<T, false, ALIGNED, 4><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
+  }
   if constexpr (!SPREAD)
     if (p.dot) return launch_dot<T, SPREAD, ALIGNED, false>(p, stream);
   return launch_status();

@@ -25,7 +25,7 @@
 #include <algorithm>
 #include <atomic>
 
-#include "common.cuh"
+#include "mbarrier.cuh"
 
 namespace tsb {
 namespace scan {
@@ -214,7 +214,6 @@ __device__ __forceinline__ int64_t part_begin(const ScanParams &p, const int64_t
 // ---- exchange between the CTAs of a cluster: values stored into a neighbour's shared memory complete bytes of a barrier
 // there, so a CTA waits for what it needs and for nothing else (a cluster-wide barrier would also wait for the outputs'
 // stores to drain: 1.2 of 7.9 cycles between two instructions of a warp went there)
-__device__ __forceinline__ unsigned smem_at(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ unsigned remote_at(unsigned addr, int rank) {
   unsigned r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
@@ -222,21 +221,6 @@ __device__ __forceinline__ unsigned remote_at(unsigned addr, int rank) {
 }
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ void mbar_init(unsigned bar) { asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ void mbar_init_done() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
-__device__ __forceinline__ void mbar_expect(unsigned bar, unsigned bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-// false if the bytes did not come within the limit (they always do: the CTAs of a cluster run together)
-__device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
-  for (int i = 0; i < (1 << 22); ++i) {
-    unsigned ok;
-    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    if (ok) return true;
-  }
-  return false;
 }
 __device__ __forceinline__ void send(unsigned addr, unsigned bar, float a, float b) {
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(addr), "f"(a), "f"(b), "r"(bar) : "memory");

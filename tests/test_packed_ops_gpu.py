@@ -151,6 +151,42 @@ def test_dispatch_and_combine(T, k, K, E, weighted, dtype):
             ref.assert_within(grads[1], dots, dots_tol, name + ' grad of the weights')
 
 
+@pytest.mark.parametrize('dtype', [F32, F16, BF16, F64])
+@pytest.mark.parametrize('weighted', [False, True])
+@pytest.mark.parametrize('T,k,K', [(2500, 1, 256), (2400, 2, 1032), (2371, 8, 520), (2400, 3, 1027), (3001, 9, 264), (2368, 33, 256)])
+def test_many_tokens(T, k, K, weighted, dtype):
+    """Tokens enough for the kernels that keep a pipeline per warp: rows of one and more pieces, ragged last pieces."""
+    gen = torch.Generator().manual_seed(T + k + K)
+    slot, indptr = plan(gen, T, k, 13)
+    few, many = rand(gen, T, K, dtype=dtype), rand(gen, T * k, K, dtype=dtype)
+    many[indptr[-1]:] = math.nan
+    acc = F64 if dtype == F64 else F32
+    weight = rand(gen, T, k, dtype=acc) if weighted else None
+    u, w64 = ref.unit(dtype), None if weight is None else weight.double()
+    # the 64-bit results by indexing, all tokens at once
+    at, named = slot.clamp_min(0), (slot >= 0).unsqueeze(-1)
+    clean = many.double().nan_to_num(0)
+    picked = clean[at] * named
+    factor = named.double() * (1 if w64 is None else w64.unsqueeze(-1))
+    fold, mass = (picked * factor).sum(1), (picked * factor).abs().sum(1)
+    spread = torch.zeros(T * k, K, dtype=torch.float64)
+    spread[slot[slot >= 0]] = (few.double().unsqueeze(1) * factor)[slot >= 0]
+    dots, dmass = (picked * few.double().unsqueeze(1)).sum(-1), (picked * few.double().unsqueeze(1)).abs().sum(-1)
+    spread_tol = (spread.abs() * u + ref.last_rounding(spread, dtype)) if weighted else torch.zeros_like(spread)
+    fold_tol = mass * u * (k + 2) + ref.last_rounding(fold, dtype)
+    for name, x, grad, call, want, want_grad, tol, grad_tol in (
+            ('dispatch', few, many, ts.expert_dispatch, spread, fold, spread_tol, fold_tol),
+            ('combine', many, few, ts.expert_combine, fold, spread, fold_tol, spread_tol)):
+        xd = x.cuda().requires_grad_()
+        wd = None if weight is None else weight.cuda().requires_grad_()
+        out = call(xd, slot.cuda(), indptr.cuda(), wd)
+        ref.assert_within(out, want, tol, name)
+        grads = torch.autograd.grad(out, (xd,) if wd is None else (xd, wd), grad.cuda())
+        ref.assert_within(grads[0], want_grad, grad_tol, name + ' grad')
+        if weighted:
+            ref.assert_within(grads[1], dots, dmass * u * (K + 2) + 1e-300, name + ' grad of the weights')
+
+
 def test_rows_of_several_dimensions_strides_and_alignment():
     gen = torch.Generator().manual_seed(3)
     slot, indptr = plan(gen, 12, 2, 4)
