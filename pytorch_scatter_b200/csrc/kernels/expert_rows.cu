@@ -272,11 +272,13 @@ __global__ void __launch_bounds__(kThreads) rows_dot_kernel(RowsParams p) {
   if constexpr (SPREAD && WRITE) zero_tail<T, ALIGNED>(p, (int64_t)blockIdx.x * kThreads + threadIdx.x, (int64_t)gridDim.x * kThreads);
 }
 
-// Long aligned rows of many tokens.  Every warp runs a pipeline of its own: bulk copies bring pieces of its tokens' rows
-// into a ring in shared memory, several steps ahead of the step that is summed, scaled or stored, so the bytes in flight
-// depend neither on registers nor on occupancy.  Lane j carries the j-th choice.  An unweighted spread only passes
-// through: bulk stores take the piece to its k places.
-constexpr int kBulkWarps = 8, kBulkMostStages = 8, kBulkWarpBytes = 12 * 1024, kBulkChunks = 4;
+// Folds, and spreads with dot products, of long aligned rows of many tokens.  Every warp runs a pipeline of its own: bulk
+// copies bring pieces of its tokens' rows into a ring in shared memory, two steps and more ahead of the step that is
+// worked on, so the bytes in flight depend neither on registers nor on occupancy.  Lane j carries the j-th choice.
+// (Combine of 32768 x 2 x 4096 bf16: 140 us against 170 with the rows in flight in registers; with the products, backward,
+// 224 against 256.  A plain spread has nothing to wait for but one load and stays with rows_kernel, 205 us against 225.)
+constexpr int kBulkWarps = 8, kBulkMostStages = 8, kBulkChunks = 2, kBulkMostDots = 8;
+constexpr int kBulkWarpBytes = 27 * 512;  // three steps of 9 pieces of 512 bytes; two CTAs fit an SM
 constexpr int kBulkSmem = kBulkWarps * kBulkWarpBytes;
 
 struct BulkShape { int piece, stages, rows; };  // bytes of a row in a step, steps in the ring, rows of a step
@@ -285,7 +287,6 @@ template <typename T, bool SPREAD, bool DOT>
 __global__ void __launch_bounds__(kBulkWarps * 32, 2) rows_bulk_kernel(RowsParams p, BulkShape shape) {
   using A = acc_t<T>;
   constexpr int V = chunk_len<T>(), U = kBulkChunks;
-  constexpr bool kFew = SPREAD || DOT, kMany = !SPREAD || DOT;
   extern __shared__ __align__(128) char s_ring[];
   __shared__ __align__(8) uint64_t s_bar[kBulkWarps][kBulkMostStages];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = (int)p.k;
@@ -315,12 +316,11 @@ __global__ void __launch_bounds__(kBulkWarps * 32, 2) rows_bulk_kernel(RowsParam
       const int64_t off = (int64_t)ipiece * shape.piece;
       const unsigned len = (unsigned)(row_bytes - off < shape.piece ? row_bytes - off : shape.piece);
       const unsigned b = bar + istage * 8, to = ring + istage * step_bytes;
-      const bool mine = kMany && islot >= 0;
-      const int rows = __popc(__ballot_sync(kFullMask, mine)) + (kFew ? 1 : 0);
+      const int rows = __popc(__ballot_sync(kFullMask, islot >= 0)) + (DOT ? 1 : 0);
       if (lane == 0) mbar_expect(b, rows * len);
       __syncwarp();
-      if (kFew && lane == 0) bulk_load(to, few_in + it * row_bytes + off, len, b);
-      if (mine) bulk_load(to + (lane + (kFew ? 1 : 0)) * shape.piece, many_in + islot * row_bytes + off, len, b);
+      if (DOT && lane == 0) bulk_load(to, few_in + it * row_bytes + off, len, b);
+      if (islot >= 0) bulk_load(to + (lane + (DOT ? 1 : 0)) * shape.piece, many_in + islot * row_bytes + off, len, b);
       if (++ipiece == pieces) {
         ipiece = 0;
         it += warps;
@@ -338,64 +338,49 @@ __global__ void __launch_bounds__(kBulkWarps * 32, 2) rows_bulk_kernel(RowsParam
     const int64_t my_slot = slot_of(t);
     const A my_weight = weight && lane < k ? weight[t * k + lane] : (A)1;
     const unsigned valid = __ballot_sync(kFullMask, my_slot >= 0);
-    A my_dot = 0;
+    A d[kBulkMostDots];
+#pragma unroll
+    for (int j = 0; j < kBulkMostDots; ++j) d[j] = 0;
     for (int q = 0; q < pieces; ++q) {
       const int64_t off = (int64_t)q * shape.piece;
       const int len = (int)(row_bytes - off < shape.piece ? row_bytes - off : shape.piece);
-      const bool came = mbar_wait(bar + stage * 8, phase);
+      const A lost = mbar_wait(bar + stage * 8, phase) ? (A)0 : (A)NAN;
       const char *at = ring_p + stage * step_bytes;
-      if constexpr (SPREAD && !DOT) {
-        if (!weight) {
-          if (my_slot >= 0 && came) bulk_store(many_out + my_slot * row_bytes + off, ring + stage * step_bytes, len);
-          bulk_commit();
-          bulk_read_done<1>();  // the step before has left its place in the ring, which issue() fills again
-          __syncwarp();
-          issue();
-          if (++stage == shape.stages) { stage = 0; phase ^= 1; }
-          continue;
-        }
-      }
       for (int c0 = lane * 16; c0 - lane * 16 < len; c0 += 32 * 16 * U) {
         Pack<T, V> few[U];
         A sum[U][V];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int c = c0 + u * 512;
-          if (kFew && c < len) few[u] = *reinterpret_cast<const Pack<T, V> *>(at + c);
-          if (SPREAD && !came) few[u] = scaled<T, A>(few[u], (A)NAN);
-          if constexpr (!SPREAD) {
+          if (DOT && c < len) few[u] = *reinterpret_cast<const Pack<T, V> *>(at + c);
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum[u][i] = came ? (A)0 : (A)NAN;
-          }
+          for (int i = 0; i < V; ++i) sum[u][i] = lost;
         }
-        for (int j = 0; j < k; ++j) {
-          if (!(valid >> j & 1)) continue;
+        const auto choice = [&](int j, A &dj) {
+          if (!(valid >> j & 1)) return;
           const A w = __shfl_sync(kFullMask, my_weight, j);
-          A d = 0;
-          const char *row = at + (j + (kFew ? 1 : 0)) * shape.piece;
+          const char *row = at + (j + (DOT ? 1 : 0)) * shape.piece;
           const int64_t to = SPREAD ? __shfl_sync(kFullMask, my_slot, j) * row_bytes + off : 0;
+          dj += lost;
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             const int c = c0 + u * 512;
             if (c >= len) continue;
-            Pack<T, V> m;
-            if constexpr (kMany) m = *reinterpret_cast<const Pack<T, V> *>(row + c);
-            if constexpr (DOT) {
+            const Pack<T, V> m = *reinterpret_cast<const Pack<T, V> *>(row + c);
+            if constexpr (SPREAD) st_stream<T, V>(reinterpret_cast<T *>(many_out + to + c), weight ? scaled<T, A>(few[u], w) : few[u]);
 #pragma unroll
-              for (int i = 0; i < V; ++i) d += to_acc<T>(few[u].v[i]) * to_acc<T>(m.v[i]);
-            }
-            if constexpr (SPREAD) {
-              st_stream<T, V>(reinterpret_cast<T *>(many_out + to + c), weight ? scaled<T, A>(few[u], w) : few[u]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < V; ++i) sum[u][i] += to_acc<T>(m.v[i]) * w;
+            for (int i = 0; i < V; ++i) {
+              const A a = to_acc<T>(m.v[i]);
+              if (DOT) dj += to_acc<T>(few[u].v[i]) * a;
+              if (!SPREAD) sum[u][i] += a * w;
             }
           }
-          if constexpr (DOT) {
+        };
+        if constexpr (DOT) {
 #pragma unroll
-            for (int s = 16; s; s >>= 1) d += shfl_xor(d, s);
-            if (lane == j) my_dot += came ? d : (A)NAN;
-          }
+          for (int j = 0; j < kBulkMostDots; ++j) choice(j, d[j]);
+        } else {
+          for (int j = 0; j < k; ++j) choice(j, d[0]);
         }
         if constexpr (!SPREAD) {
 #pragma unroll
@@ -413,22 +398,28 @@ __global__ void __launch_bounds__(kBulkWarps * 32, 2) rows_bulk_kernel(RowsParam
       issue();
       if (++stage == shape.stages) { stage = 0; phase ^= 1; }
     }
-    if (DOT && lane < k) static_cast<A *>(p.dot)[t * k + lane] = my_dot;
+    if constexpr (DOT) {
+      A mine = 0;
+#pragma unroll
+      for (int j = 0; j < kBulkMostDots; ++j) {
+#pragma unroll
+        for (int s = 16; s; s >>= 1) d[j] += shfl_xor(d[j], s);
+        if (lane == j) mine = d[j];
+      }
+      if (lane < k) static_cast<A *>(p.dot)[t * k + lane] = mine;
+    }
   }
-  if constexpr (SPREAD) {
-    zero_tail<T, true>(p, (int64_t)blockIdx.x * kBulkWarps * 32 + threadIdx.x, (int64_t)gridDim.x * kBulkWarps * 32);
-    bulk_read_done<0>();
-  }
+  if constexpr (SPREAD) zero_tail<T, true>(p, (int64_t)blockIdx.x * kBulkWarps * 32 + threadIdx.x, (int64_t)gridDim.x * kBulkWarps * 32);
 }
 
-// Whether the pipeline takes the problem: enough tokens for every warp to have some, rows of 512 bytes and more, and at
-// least three steps in the ring.
-template <typename T, bool SPREAD, bool DOT> bool bulk_shape(const RowsParams &p, BulkShape &s) {
+// Whether the pipeline takes the problem: enough tokens for every warp to have some, rows of 512 bytes and more, a lane
+// for each choice (and a register for its product), and at least three steps in the ring.
+template <typename T, bool DOT> bool bulk_shape(const RowsParams &p, BulkShape &s) {
   const int64_t row_bytes = p.K * (int64_t)sizeof(T);
-  if (p.k > 32 || row_bytes < 512 || row_bytes > 1 << 30 || p.T < (int64_t)sm_count() * kBulkWarps * 2) return false;
-  s.rows = (SPREAD || DOT ? 1 : 0) + (!SPREAD || DOT ? (int)p.k : 0);
+  if (p.k > (DOT ? kBulkMostDots : 32) || row_bytes < 512 || row_bytes > 1 << 30 || p.T < (int64_t)sm_count() * kBulkWarps * 2) return false;
+  s.rows = (int)p.k + (DOT ? 1 : 0);
   s.piece = 4096;
-  while (s.piece > 512 && (s.piece > row_bytes || s.rows * s.piece * 4 > kBulkWarpBytes)) s.piece /= 2;
+  while (s.piece > 512 && (s.piece > row_bytes || s.rows * s.piece * 3 > kBulkWarpBytes)) s.piece /= 2;
   s.stages = std::min(kBulkMostStages, kBulkWarpBytes / (s.rows * s.piece));
   return s.stages >= 3;
 }
@@ -470,8 +461,9 @@ template <typename T, bool SPREAD, bool ALIGNED, bool WRITE> int launch_dot(cons
 template <typename T, bool SPREAD, bool ALIGNED> int launch_rows(const RowsParams &p, cudaStream_t stream) {
   if constexpr (ALIGNED) {
     BulkShape shape;
-    if (p.dot ? bulk_shape<T, SPREAD, true>(p, shape) : bulk_shape<T, SPREAD, false>(p, shape))
-      return p.dot ? launch_bulk<T, SPREAD, true>(p, shape, stream) : launch_bulk<T, SPREAD, false>(p, shape, stream);
+    if (p.dot && bulk_shape<T, true>(p, shape)) return launch_bulk<T, SPREAD, true>(p, shape, stream);
+    if constexpr (!SPREAD)
+      if (!p.dot && bulk_shape<T, false>(p, shape)) return launch_bulk<T, false, false>(p, shape, stream);
   }
   if (p.dot && (SPREAD || p.k <= 8)) return launch_dot<T, SPREAD, ALIGNED, true>(p, stream);
   const int64_t items = p.T * chunks_of<T, ALIGNED>(p.K);

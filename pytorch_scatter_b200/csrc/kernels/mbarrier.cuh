@@ -1,4 +1,4 @@
-// Shared-memory barriers that count arriving bytes (mbarrier), and the bulk copies that complete them.
+// Shared-memory barriers that count arriving bytes (mbarrier), and the bulk loads that complete them.
 #pragma once
 
 #include "common.cuh"
@@ -27,11 +27,4 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
 __device__ __forceinline__ void bulk_load(unsigned dst, const void *src, unsigned bytes, unsigned bar) {
   asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void bulk_store(void *dst, unsigned src, unsigned bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-// the calling thread's bulk stores, all but the N youngest groups, have read their source
-template <int N> __device__ __forceinline__ void bulk_read_done() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
-
 }  // namespace tsb
