@@ -32,7 +32,48 @@ template <typename T> constexpr int chunk_len() { return 16 / (int)sizeof(T); }
 // elements [a, b) of a chunk belong to the row
 struct Span { int a, b; };
 
-// V elements from p on, wherever p is; those outside the span are 0.  lo, hi: the ends of the array p points into.
+// V elements from p on, wherever p is; those outside the span are 0.  The loads are issued here, so that those of several
+// rows are in flight at once, and read() shifts the elements into place.  lo, hi: the ends of the array p points into; a
+// chunk whose two aligned halves are not both inside is read element by element.
+template <typename T> struct AnyChunk {
+  static constexpr int V = chunk_len<T>();
+  uint4 x, y;
+  const T *p;
+  Span s;
+  int off;  // -1: element by element
+  __device__ __forceinline__ void load(const T *p_, Span s_, const T *lo, const T *hi) {
+    p = p_;
+    s = s_;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p), base = at & ~(uintptr_t)15;
+    off = (int)(at & 15);
+    const bool inside = base >= reinterpret_cast<uintptr_t>(lo) && base + 32 <= reinterpret_cast<uintptr_t>(hi);
+    if (s.a == 0 && s.b == V && (off == 0 || inside)) {
+      x = *reinterpret_cast<const uint4 *>(base);
+      y = *reinterpret_cast<const uint4 *>(base + (off ? 16 : 0));
+    } else {
+      off = -1;
+    }
+  }
+  __device__ __forceinline__ Pack<T, V> read() const {
+    Pack<T, V> r;
+    if (off >= 0) {
+      unsigned w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int i = 0; i < 6; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], off & 2 ? 16 : 0);
+      return *reinterpret_cast<const Pack<T, V> *>(w);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = i >= s.a && i < s.b ? p[i] : from_acc<T>((acc_t<T>)0);
+    return r;
+  }
+};
+// The same, loaded and shifted at once: where occupancy hides the latency, fewer registers and the branches that spare the
+// second load and the shifts win (fold of 16384 x 4 x 2047 bf16: 162 us, 217 with all loads first; with dot products it
+// is the other way round, 303 and 237).
 template <typename T>
 __device__ __forceinline__ Pack<T, chunk_len<T>()> load_any(const T *p, Span s, const T *lo, const T *hi) {
   constexpr int V = chunk_len<T>();
@@ -62,6 +103,14 @@ __device__ __forceinline__ Pack<T, chunk_len<T>()> load_any(const T *p, Span s, 
   for (int i = 0; i < V; ++i) r.v[i] = i >= s.a && i < s.b ? p[i] : from_acc<T>((acc_t<T>)0);
   return r;
 }
+template <typename T> struct AlignedChunk {
+  static constexpr int V = chunk_len<T>();
+  Pack<T, V> v;
+  __device__ __forceinline__ void load(const T *p, Span, const T *, const T *) { v = ld_stream<T, V>(p); }
+  __device__ __forceinline__ Pack<T, V> read() const { return v; }
+};
+template <typename T, bool ALIGNED> using Chunk = std::conditional_t<ALIGNED, AlignedChunk<T>, AnyChunk<T>>;
+
 template <typename T> __device__ __forceinline__ void store_span(T *p, const Pack<T, chunk_len<T>()> &v, Span s) {
   constexpr int V = chunk_len<T>();
   if (s.a == 0 && s.b == V) {
@@ -90,11 +139,6 @@ template <typename T, bool ALIGNED> __host__ __device__ __forceinline__ int64_t 
   constexpr int V = chunk_len<T>();
   return ALIGNED ? K / V : (K + 2 * V - 2) / V;
 }
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ Pack<T, chunk_len<T>()> load_chunk(const T *row, int64_t e0, Span s, const T *lo, const T *hi) {
-  if constexpr (ALIGNED) return ld_stream<T, chunk_len<T>()>(row + e0);
-  else return load_any<T>(row + e0, s, lo, hi);
-}
 template <typename T, typename A> __device__ __forceinline__ Pack<T, chunk_len<T>()> scaled(const Pack<T, chunk_len<T>()> &v, A w) {
   Pack<T, chunk_len<T>()> o;
 #pragma unroll
@@ -114,10 +158,10 @@ template <typename T, bool ALIGNED> __device__ __forceinline__ void zero_tail(co
 }
 
 // Without dot products: one thread, one chunk of one token.  The rows of several choices are in flight at once.
-template <typename T, bool SPREAD, bool ALIGNED, int J>
+template <typename T, bool SPREAD, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
   using A = acc_t<T>;
-  constexpr int V = chunk_len<T>();
+  constexpr int V = chunk_len<T>(), J = 4;
   const A *__restrict__ weight = static_cast<const A *>(p.weight);
   const T *few_in = static_cast<const T *>(p.few_in), *many_in = static_cast<const T *>(p.many_in);
   T *few_out = static_cast<T *>(p.few_out), *many_out = static_cast<T *>(p.many_out);
@@ -128,18 +172,24 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
     const int64_t *slot = p.slot + t * p.k;
     Span s;
     if constexpr (SPREAD) {
-      Pack<T, V> v;
-      if constexpr (ALIGNED) v = ld_stream<T, V>(few_in + t * p.K + c * V);
-      for (int64_t j = 0; j < p.k; ++j) {
-        const int64_t to = slot[j];
-        if (to < 0 || to >= p.M) continue;
-        T *row = many_out + to * p.K;
-        const int64_t e0 = chunk_of<T, ALIGNED>(row, c, p.K, s);
-        if constexpr (!ALIGNED) {
-          if (s.b <= s.a) continue;
-          v = load_any<T>(few_in + t * p.K + e0, s, few_in, few_in + p.T * p.K);
+      if constexpr (ALIGNED) {
+        s = {0, V};
+        const Pack<T, V> v = ld_stream<T, V>(few_in + t * p.K + c * V);
+        for (int64_t j = 0; j < p.k; ++j) {
+          const int64_t to = slot[j];
+          if (to < 0 || to >= p.M) continue;
+          store_span<T>(many_out + to * p.K + c * V, weight ? scaled<T, A>(v, weight[t * p.k + j]) : v, s);
         }
-        store_span<T>(row + e0, weight ? scaled<T, A>(v, weight[t * p.k + j]) : v, s);
+      } else {
+        for (int64_t j = 0; j < p.k; ++j) {
+          const int64_t to = slot[j];
+          if (to < 0 || to >= p.M) continue;
+          T *row = many_out + to * p.K;
+          const int64_t e0 = chunk_of<T, false>(row, c, p.K, s);
+          if (s.b <= s.a) continue;
+          const Pack<T, V> v = load_any<T>(few_in + t * p.K + e0, s, few_in, few_in + p.T * p.K);
+          store_span<T>(row + e0, weight ? scaled<T, A>(v, weight[t * p.k + j]) : v, s);
+        }
       }
     } else {
       T *row = few_out + t * p.K;
@@ -155,7 +205,9 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
         for (int j = 0; j < J; ++j) {
           const int64_t from = j0 + j < p.k ? slot[j0 + j] : -1;
           some[j] = from >= 0 && from < p.M;
-          if (some[j]) v[j] = load_chunk<T, ALIGNED>(many_in + from * p.K, e0, s, many_in, many_in + p.M * p.K);
+          if (!some[j]) continue;
+          if constexpr (ALIGNED) v[j] = ld_stream<T, V>(many_in + from * p.K + e0);
+          else v[j] = load_any<T>(many_in + from * p.K + e0, s, many_in, many_in + p.M * p.K);
         }
 #pragma unroll
         for (int j = 0; j < J; ++j) {
@@ -175,7 +227,8 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
 }
 
 // With dot products: G threads (lanes of a warp, or the CTA) walk one token's chunks, J choices at a time.  WRITE: also
-// spread or fold; a fold needs all choices of a chunk at once, so it has J >= k.
+// spread or fold; a fold needs all choices of a chunk at once, so it has J >= k.  Unaligned chunks take
+// twice the registers, so fewer choices are in flight.
 template <typename T, bool SPREAD, bool ALIGNED, bool WRITE, int J, int G>
 __global__ void __launch_bounds__(kThreads) rows_dot_kernel(RowsParams p) {
   using A = acc_t<T>;
@@ -204,36 +257,39 @@ __global__ void __launch_bounds__(kThreads) rows_dot_kernel(RowsParams p) {
       if (live) {
         const T *few = few_in + t * p.K;
         for (int64_t c = lane; c < Kc; c += G) {
-          Pack<T, V> x, y[J];
-          Span s;
-          int64_t e0 = 0;
-          if constexpr (ALIGNED || !SPREAD) {
-            e0 = chunk_of<T, ALIGNED>(SPREAD || !WRITE ? few : few_out + t * p.K, c, p.K, s);
-            if (!ALIGNED && s.b <= s.a) continue;
-            x = load_chunk<T, ALIGNED>(few, e0, s, few_in, few_in + p.T * p.K);
-          }
-          A fold[V];
-#pragma unroll
-          for (int i = 0; i < V; ++i) fold[i] = 0;
-          if constexpr (ALIGNED || !SPREAD) {
-#pragma unroll
-            for (int j = 0; j < J; ++j)
-              if (at[j] >= 0) y[j] = load_chunk<T, ALIGNED>(many_in + at[j] * p.K, e0, s, many_in, many_in + p.M * p.K);
+          // the chunks of the row that is written; with many rows written and no alignment, those of each choice's row
+          constexpr bool kEach = SPREAD && !ALIGNED;
+          Chunk<T, ALIGNED> x[kEach ? J : 1], y[J];
+          Span s[kEach ? J : 1];
+          int64_t e0[kEach ? J : 1];
+          if constexpr (!kEach) {
+            e0[0] = chunk_of<T, ALIGNED>(SPREAD || !WRITE ? few : few_out + t * p.K, c, p.K, s[0]);
+            if (!ALIGNED && s[0].b <= s[0].a) continue;
+            x[0].load(few + e0[0], s[0], few_in, few_in + p.T * p.K);
           }
 #pragma unroll
           for (int j = 0; j < J; ++j) {
             if (at[j] < 0) continue;
-            if constexpr (!ALIGNED && SPREAD) {  // the chunks of this choice's row
-              e0 = chunk_of<T, false>(many_out + at[j] * p.K, c, p.K, s);
-              if (s.b <= s.a) continue;
-              x = load_any<T>(few + e0, s, few_in, few_in + p.T * p.K);
-              y[j] = load_any<T>(many_in + at[j] * p.K + e0, s, many_in, many_in + p.M * p.K);
+            if constexpr (kEach) {
+              e0[j] = chunk_of<T, false>(many_out + at[j] * p.K, c, p.K, s[j]);
+              if (s[j].b <= s[j].a) continue;
+              x[j].load(few + e0[j], s[j], few_in, few_in + p.T * p.K);
             }
-            if constexpr (SPREAD && WRITE) store_span<T>(many_out + at[j] * p.K + e0, weight ? scaled<T, A>(x, w[j]) : x, s);
+            y[j].load(many_in + at[j] * p.K + e0[kEach ? j : 0], s[kEach ? j : 0], many_in, many_in + p.M * p.K);
+          }
+          A fold[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) fold[i] = 0;
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            const Span sj = s[kEach ? j : 0];
+            if (at[j] < 0 || (!ALIGNED && sj.b <= sj.a)) continue;
+            const Pack<T, V> xv = x[kEach ? j : 0].read(), yv = y[j].read();
+            if constexpr (SPREAD && WRITE) store_span<T>(many_out + at[j] * p.K + e0[kEach ? j : 0], weight ? scaled<T, A>(xv, w[j]) : xv, sj);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-              const A a = to_acc<T>(y[j].v[i]);
-              sum[j] += to_acc<T>(x.v[i]) * a;
+              const A a = to_acc<T>(yv.v[i]);
+              sum[j] += to_acc<T>(xv.v[i]) * a;
               if (!SPREAD && WRITE) fold[i] += a * w[j];
             }
           }
@@ -241,7 +297,7 @@ __global__ void __launch_bounds__(kThreads) rows_dot_kernel(RowsParams p) {
             Pack<T, V> o;
 #pragma unroll
             for (int i = 0; i < V; ++i) o.v[i] = from_acc<T>(fold[i]);
-            store_span<T>(few_out + t * p.K + e0, o, s);
+            store_span<T>(few_out + t * p.K + e0[0], o, s[0]);
           }
         }
       }
@@ -445,11 +501,10 @@ template <typename T, bool SPREAD, bool ALIGNED, bool WRITE> int launch_dot(cons
     return launch_status();
   };
   const auto with_j = [&](auto gn) {
-    if constexpr (WRITE) {  // (the products alone are only asked for where there are more than eight choices)
-      if (p.k <= 2) return go(std::integral_constant<int, 2>(), gn);
-      if (p.k <= 4) return go(std::integral_constant<int, 4>(), gn);
-    }
-    return go(std::integral_constant<int, 8>(), gn);
+    if (p.k <= 2 || (SPREAD && !ALIGNED)) return go(std::integral_constant<int, 2>(), gn);
+    if constexpr (ALIGNED && WRITE)
+      if (p.k > 4) return go(std::integral_constant<int, 8>(), gn);
+    return go(std::integral_constant<int, 4>(), gn);
   };
   // Threads of a token: what its chunks keep busy, and a whole CTA where the tokens alone would not fill the GPU.
   const int64_t Kc = chunks_of<T, ALIGNED>(p.K);
@@ -465,15 +520,10 @@ template <typename T, bool SPREAD, bool ALIGNED> int launch_rows(const RowsParam
     if constexpr (!SPREAD)
       if (!p.dot && bulk_shape<T, false>(p, shape)) return launch_bulk<T, false, false>(p, shape, stream);
   }
-  if (p.dot && (SPREAD || p.k <= 8)) return launch_dot<T, SPREAD, ALIGNED, true>(p, stream);
+  if (p.dot && (SPREAD || p.k <= (ALIGNED ? 8 : 4))) return launch_dot<T, SPREAD, ALIGNED, true>(p, stream);
   const int64_t items = p.T * chunks_of<T, ALIGNED>(p.K);
   const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((int64_t)sm_count() * 64, (items + kThreads - 1) / kThreads));
-  if constexpr (SPREAD) {
-    rows_kernel<T, true, ALIGNED, 1><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
-  } else {
-    if (p.k <= 2) rows_kernel<T, false, ALIGNED, 2><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
-    else rows_kernel<T, false, ALIGNED, 4><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
-  }
+  rows_kernel<T, SPREAD, ALIGNED><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
   if constexpr (!SPREAD)
     if (p.dot) return launch_dot<T, SPREAD, ALIGNED, false>(p, stream);
   return launch_status();
