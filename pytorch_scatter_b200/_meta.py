@@ -142,12 +142,13 @@ if _lib_defined:
         return src.new_empty(shape, dtype=_acc_dtype(src))
 
     @torch.library.register_fake('torch_scatter::_scan_csr_fw')
-    def _(src, gate, indptr, state, want_last):
+    def _(src, gate, indptr, state, want_last, want_wide):
         out = torch.empty_like(src, memory_format=torch.contiguous_format)
-        return out, _states(src, indptr) if want_last else _placeholder(src)
+        return (out, _states(src, indptr) if want_last else _placeholder(src),
+                src.new_empty(src.shape, dtype=_acc_dtype(src)) if want_wide else _placeholder(src))
 
     @torch.library.register_fake('torch_scatter::_scan_csr_bw')
-    def _(grad_out, grad_last, gate, out, indptr, state, want_gate, want_state):
+    def _(grad_out, grad_last, gate, out, wide, indptr, state, want_gate, want_state):
         return (torch.empty_like(out, memory_format=torch.contiguous_format),
                 torch.empty_like(gate, memory_format=torch.contiguous_format) if want_gate else _placeholder(gate),
                 _states(out, indptr) if want_state else _placeholder(out))

@@ -53,13 +53,14 @@ using namespace tsb;
 extern "C" size_t tsb_scan_csr_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int, int) { return 0; }
 
 extern "C" int tsb_scan_csr(const void *src, const void *gate, const int64_t *indptr, const void *state, void *out, void *last,
-                            int64_t B, int64_t E, int64_t K, int64_t N, int64_t width, int64_t indptr_batch_stride, int dtype,
+                            void *wide, int64_t B, int64_t E, int64_t K, int64_t N, int64_t width, int64_t indptr_batch_stride, int dtype,
                             int gate_dtype, void *, size_t, tsb_stream_t stream) {
   if (const int st = check(B, E, K, N, width, dtype, gate_dtype)) return st;
   if (B == 0 || K == 0 || (E == 0 && (N == 0 || !last))) return TSB_OK;
   if (!indptr || (E > 0 && (!src || !gate || !out))) return TSB_ERR_ARG;
   ScanParams p{};
-  p.src = src; p.gate = gate; p.state = state; p.indptr = indptr; p.out = out; p.last = last;
+  if (wide && gate_dtype == dtype) return TSB_ERR_ARG;
+  p.src = src; p.gate = gate; p.state = state; p.indptr = indptr; p.out = out; p.last = last; p.wide = wide;
   p.B = B; p.E = E; p.K = K; p.N = N; p.width = width; p.bstride = indptr_batch_stride;
   return launch_tiles(p, dtype, gate_dtype, false, stream);
 }
@@ -69,17 +70,17 @@ extern "C" size_t tsb_scan_csr_backward_workspace_bytes(int64_t B, int64_t E, in
   return (size_t)(B * E * scan::partials_of_row(K, width, dtype_elem_bytes(dtype))) * dtype_acc_bytes(dtype);
 }
 
-extern "C" int tsb_scan_csr_backward(const void *grad_out, const void *grad_last, const void *gate, const void *out,
+extern "C" int tsb_scan_csr_backward(const void *grad_out, const void *grad_last, const void *gate, const void *h,
                                      const int64_t *indptr, const void *state, void *grad_src, void *grad_gate, void *grad_state,
                                      int64_t B, int64_t E, int64_t K, int64_t N, int64_t width, int64_t indptr_batch_stride,
                                      int dtype, int gate_dtype, void *workspace, size_t workspace_bytes, tsb_stream_t stream) {
   if (const int st = check(B, E, K, N, width, dtype, gate_dtype)) return st;
   if (B == 0 || K == 0 || (E == 0 && (N == 0 || !grad_state))) return TSB_OK;
-  if (!indptr || (E > 0 && (!gate || !out || !grad_src))) return TSB_ERR_ARG;
+  if (!indptr || (E > 0 && (!gate || (grad_gate && !h) || !grad_src))) return TSB_ERR_ARG;
   const size_t need = grad_gate && E > 0 ? tsb_scan_csr_backward_workspace_bytes(B, E, K, N, width, dtype, gate_dtype) : 0;
   if (need > 0 && (!workspace || workspace_bytes < need)) return TSB_ERR_WORKSPACE;
   ScanParams p{};
-  p.src = grad_out; p.gate = gate; p.state = grad_last; p.fwd = out; p.init = state; p.indptr = indptr;
+  p.src = grad_out; p.gate = gate; p.state = grad_last; p.fwd = h; p.init = state; p.indptr = indptr;
   p.out = grad_src; p.last = grad_state; p.grad_gate = grad_gate; p.partial = workspace;
   p.B = B; p.E = E; p.K = K; p.N = N; p.width = width; p.bstride = indptr_batch_stride;
   return launch_tiles(p, dtype, gate_dtype, true, stream);

@@ -37,10 +37,11 @@ constexpr int kMostCluster = 8;
 
 struct ScanParams {
   const void *src, *gate, *state;  // backward: src = grad_out (may be null), state = grad_last
-  const void *fwd, *init;          // backward: the forward's out and state
+  const void *fwd, *init;          // backward: the forward's h and state
   const int64_t *indptr;
   void *out, *last;                // backward: grad_src, grad_state
   void *grad_gate, *partial;       // backward
+  void *wide;                      // forward: h in the accumulation type as well, or null
   int64_t B, E, K, N, width, bstride;
   int64_t parts, tiles_k;
   int lx_log2, cluster, lanes_log2;  // lanes_log2: lanes of one row whose gate products are summed by shuffles
@@ -51,15 +52,15 @@ constexpr int kStart = 1, kEnd = 2, kDead = 4, kPad = 8, kMarkBits = 4;
 constexpr int64_t kMostSegments = (int64_t)1 << 27;
 
 // A copy of VEC values to the thread's own slot.  One 2-byte value travels in the 4-byte word that holds it (cp.async has
-// no smaller form), unless that word reaches over the array's ends; `half` says which half it is.
+// no smaller form), unless that word reaches over the array's ends (`edge`: it may); `half` says which half it is.
 template <typename T, int VEC> struct Slot {
   static constexpr bool kWord = sizeof(T) * VEC == 2;
   static constexpr int kBytes = kWord ? 4 : (int)sizeof(T) * VEC;
   static __device__ __forceinline__ int half(const T *p) { return kWord ? (int)(reinterpret_cast<uintptr_t>(p) >> 1) & 1 : 0; }
-  static __device__ __forceinline__ void copy(char *slot, const T *p, const T *lo, const T *hi) {
+  static __device__ __forceinline__ void copy(char *slot, const T *p, bool edge, const T *lo, const T *hi) {
     if constexpr (kWord) {
       const uintptr_t word = reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3;
-      if (word >= reinterpret_cast<uintptr_t>(lo) && word + 4 <= reinterpret_cast<uintptr_t>(hi)) {
+      if (!edge || (word >= reinterpret_cast<uintptr_t>(lo) && word + 4 <= reinterpret_cast<uintptr_t>(hi))) {
         const unsigned dst = (unsigned)__cvta_generic_to_shared(slot);
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(word) : "memory");
       } else {
@@ -100,6 +101,17 @@ template <typename A, int VEC> __device__ __forceinline__ void put(A *p, const A
 #pragma unroll
     for (int j = 0; j < n; ++j) q.v[j] = v[i + j];
     *reinterpret_cast<Pack<A, n> *>(p + i) = q;
+  }
+}
+// to global memory, which is 16-byte aligned where there are as many
+template <typename A, int VEC> __device__ __forceinline__ void store_wide(A *p, const A (&v)[VEC]) {
+  constexpr int n = VEC * sizeof(A) >= 16 ? 16 / (int)sizeof(A) : 1;
+#pragma unroll
+  for (int i = 0; i < VEC; i += n) {
+    Pack<A, n> q;
+#pragma unroll
+    for (int j = 0; j < n; ++j) q.v[j] = v[i + j];
+    st_stream<A, n>(p + i, q);
   }
 }
 template <typename A, int VEC> __device__ __forceinline__ void take(A (&v)[VEC], const A *p) {
@@ -231,9 +243,14 @@ __device__ __forceinline__ void send(unsigned addr, unsigned bar, double a, doub
 template <typename T, typename G, int VEC, bool SHARED, bool BWD> struct ScanShape {
   using A = acc_t<T>;
   static constexpr int kGateVec = SHARED ? 1 : VEC;
+  // The backward multiplies dh by the h before it.  With a gate of the data's type that is the rounded output: the
+  // gradient, which is rounded to the same type, then carries two such roundings.  A wider gate has a gradient in 32 bits,
+  // which the rounding of h would spoil: its backward reads h as the recurrence held it.
+  using F = std::conditional_t<(sizeof(G) > sizeof(T)), A, T>;
   using SrcSlot = Slot<T, VEC>;
   using GateSlot = Slot<G, kGateVec>;
-  static constexpr int kRowBytes = SrcSlot::kBytes * (BWD ? 2 : 1) + GateSlot::kBytes;
+  using FwdSlot = Slot<F, VEC>;
+  static constexpr int kRowBytes = SrcSlot::kBytes + (BWD ? FwdSlot::kBytes : 0) + GateSlot::kBytes;
   // Rows of a thread: 42 KB for each of the two stages at most, so that two CTAs fit an SM.  What a tile costs besides its
   // rows, step (2), is then a small part (65536 x 4096 bf16: 291 us with 10 rows and 2 stages, 302 with 7 rows and 3
   // stages, 391 with 5 rows, 2 stages and four CTAs).
@@ -253,9 +270,12 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
   using S = ScanShape<T, G, VEC, SHARED, BWD>;
   using SrcSlot = typename S::SrcSlot;
   using GateSlot = typename S::GateSlot;
+  using FwdSlot = typename S::FwdSlot;
+  using F = typename S::F;
   using A = acc_t<T>;
   constexpr int R = S::kRows;
-  constexpr int kSrcRow = kScanThreads * SrcSlot::kBytes, kGateRow = kScanThreads * GateSlot::kBytes;
+  constexpr int kSrcRow = kScanThreads * SrcSlot::kBytes, kGateRow = kScanThreads * GateSlot::kBytes,
+                kFwdRow = kScanThreads * FwdSlot::kBytes;
 
   const int tid = threadIdx.x;
   const int lx = 1 << p.lx_log2, C = lx * VEC, L = (kScanThreads >> p.lx_log2) * R;
@@ -348,19 +368,21 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
   const int64_t srow = b * p.N;                     // first row of this batch in the state arrays
   const bool have_src = !BWD || p.src, want_gate = BWD && p.grad_gate;
   const T *src_lo = static_cast<const T *>(p.src), *src_hi = src_lo + p.B * p.E * p.K;
-  const T *fwd_lo = static_cast<const T *>(p.fwd), *fwd_hi = fwd_lo + p.B * p.E * p.K;
+  const F *fwd_lo = static_cast<const F *>(p.fwd), *fwd_hi = fwd_lo + p.B * p.E * p.K;
   const G *gate_lo = static_cast<const G *>(p.gate), *gate_hi = gate_lo + p.B * p.E * gates;
 
   // this thread's slots [stage][row][thread], and its pointers to the next tile to load and to the tile at work
   char *s_src = smem + tid * SrcSlot::kBytes;
-  char *s_fwd = s_src + kStages * R * kSrcRow;
-  char *s_gate = smem + kStages * R * kSrcRow * (BWD ? 2 : 1) + tid * GateSlot::kBytes;
+  char *s_fwd = smem + kStages * R * kSrcRow + tid * FwdSlot::kBytes;
+  char *s_gate = smem + kStages * R * (kSrcRow + (BWD ? kFwdRow : 0)) + tid * GateSlot::kBytes;
   int64_t tile = (int64_t)rank * L;                 // position of the CTA's tile
   int64_t ahead = tile + ty * R;                    // position of the thread's next rows to load
   const int64_t at = b * p.E + row_of(ahead);
-  const T *lsrc = src_lo + (have_src ? at * p.K + c0 : 0), *lfwd = fwd_lo + (BWD ? (at - 1) * p.K + c0 : 0);  // fwd: h of the row before
+  const T *lsrc = src_lo + (have_src ? at * p.K + c0 : 0);
+  const F *lfwd = fwd_lo + (BWD ? (at - 1) * p.K + c0 : 0);  // h of the row before
   const G *lgate = gate_lo + at * gates + g0;
   T *os = static_cast<T *>(p.out) + at * p.K + c0;
+  A *ow = static_cast<A *>(p.wide) + (!BWD && p.wide ? at * p.K + c0 : 0);
   G *og = static_cast<G *>(p.grad_gate) + (want_gate ? at * gates + g0 : 0);
   // sums of a shared gate's products: all of them, or what this tile's lanes hold
   const int sum_lanes = SHARED ? 1 << p.lanes_log2 : 1;
@@ -370,22 +392,26 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
   const int64_t tile_k = step * dk, tile_gates = step * dgates;
   // which half of its word a row's value is in (2-byte slots only)
   const int kodd = (int)(p.K & 1), godd = (int)(gates & 1);
-  int xhalf = SrcSlot::half(lsrc), fhalf = SrcSlot::half(lfwd), ghalf = GateSlot::half(lgate);
+  int xhalf = SrcSlot::half(lsrc), fhalf = FwdSlot::half(lfwd), ghalf = GateSlot::half(lgate);
   const int xturn = (int)(tile_k & 1), gturn = (int)(tile_gates & 1);
 
   const auto load_rows = [&](int stage) {
     const int64_t left = len - ahead;
     if (live && left > 0) {
-      const T *xs = lsrc, *fs = lfwd;
+      const T *xs = lsrc;
+      const F *fs = lfwd;
       const G *gs = lgate;
-      char *xd = s_src + stage * (R * kSrcRow), *fd = s_fwd + stage * (R * kSrcRow), *gd = s_gate + stage * (R * kGateRow);
+      char *xd = s_src + stage * (R * kSrcRow), *fd = s_fwd + stage * (R * kFwdRow), *gd = s_gate + stage * (R * kGateRow);
       const int n = left < R ? (int)left : R;
+      // only the first and the last row of the whole array hold words that reach over its ends
+      const int64_t row = b * p.E + row_of(ahead);
+      const bool edge = BWD ? row <= R || row >= p.B * p.E - 1 : row <= 0 || row + R >= p.B * p.E;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (r < n) {
-          if (have_src) SrcSlot::copy(xd + r * kSrcRow, xs, src_lo, src_hi);
-          GateSlot::copy(gd + r * kGateRow, gs, gate_lo, gate_hi);
-          if (BWD && want_gate && fs >= fwd_lo) SrcSlot::copy(fd + r * kSrcRow, fs, fwd_lo, fwd_hi);  // (row 0 has none before it)
+          if (have_src) SrcSlot::copy(xd + r * kSrcRow, xs, edge, src_lo, src_hi);
+          GateSlot::copy(gd + r * kGateRow, gs, edge, gate_lo, gate_hi);
+          if (BWD && want_gate && fs >= fwd_lo) FwdSlot::copy(fd + r * kFwdRow, fs, edge, fwd_lo, fwd_hi);  // (row 0 has none before it)
         }
         xs += dk;
         fs += dk;
@@ -420,7 +446,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
       mine = __any_sync(kFullMask, any != 0);
     }
     const char *xs = s_src + stage * (R * kSrcRow), *gs = s_gate + stage * (R * kGateRow);
-    [[maybe_unused]] const char *fs = s_fwd + stage * (R * kSrcRow);
+    [[maybe_unused]] const char *fs = s_fwd + stage * (R * kFwdRow);
     const auto read_row = [&](A (&x)[VEC], A (&g)[VEC], int r) {
       widen<T, VEC>(x, SrcSlot::get(xs + r * kSrcRow, (xhalf + r * kodd) & 1));
       if constexpr (SHARED) {
@@ -545,10 +571,11 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
     A v_[VEC];
     take(v_, s_a + own_map);
     T *orow = os;
+    A *wrow = ow;
     G *grow = og;
     A *prow = op;
 #pragma unroll
-    for (int r = 0; r < R; ++r, orow += dk, grow += dgates, prow += dsums) {
+    for (int r = 0; r < R; ++r, orow += dk, wrow += dk, grow += dgates, prow += dsums) {
       int m = 0;
       if constexpr (MARKED) {
         m = mark[r];
@@ -572,6 +599,8 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
         round_pack(o, v_);
         if (live) {
           st_stream<T, VEC>(orow, o);
+          if constexpr (!std::is_same<F, T>::value)
+            if (p.wide) store_wide(wrow, v_);
           if (MARKED && (m & kEnd) && p.last) store_acc<A, VEC>(v_, p.last, (srow + (m >> kMarkBits)) * p.K + c0);
         }
       } else {
@@ -587,7 +616,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
         if (live) st_stream<T, VEC>(orow, o);
         if (want_gate) {
           A before[VEC];
-          widen<T, VEC>(before, SrcSlot::get(fs + r * kSrcRow, (fhalf + r * kodd) & 1));
+          widen<F, VEC>(before, FwdSlot::get(fs + r * kFwdRow, (fhalf + r * kodd) & 1));
           if (MARKED && (m & (kStart | kDead))) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) before[v] = 0;
@@ -635,6 +664,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
     tile_work(stage, par, set);
     tile += step;
     os += tile_k;
+    ow += tile_k;
     og += tile_gates;
     op += step * dsums;
     xhalf ^= xturn;
@@ -776,7 +806,7 @@ inline int64_t partials_of_row(int64_t K, int64_t width, size_t elem) {
 
 template <typename T, typename G, bool BWD> int launch(const ScanParams &p, cudaStream_t stream) {
   using A = acc_t<T>;
-  const void *all[] = {p.src, p.width == 1 ? p.gate : nullptr, p.fwd, p.out, p.width == 1 ? p.grad_gate : nullptr};
+  const void *all[] = {p.src, p.width == 1 ? p.gate : nullptr, p.fwd, p.out, p.wide, p.width == 1 ? p.grad_gate : nullptr};
   bool a16 = true, a4 = true;
   for (const void *q : all) {
     a16 = a16 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;

@@ -35,31 +35,34 @@ torch::Tensor expand_indptr(const torch::Tensor &indptr, const torch::Tensor &sr
   return indptr.expand(sizes);
 }
 
-// (out, last or a placeholder)
-std::tuple<torch::Tensor, torch::Tensor> scan_fw_impl(torch::Tensor src_, torch::Tensor gate_, torch::Tensor indptr,
-                                                      std::optional<torch::Tensor> state_, bool want_last) {
+// (out, last, h in the accumulation type); the last two are placeholders where they are not wanted
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> scan_fw_impl(torch::Tensor src_, torch::Tensor gate_, torch::Tensor indptr,
+                                                                     std::optional<torch::Tensor> state_, bool want_last, bool want_wide) {
   c10::cuda::CUDAGuard guard(src_.device());
   auto src = src_.contiguous(), gate = gate_.contiguous();
   auto state = opt_contiguous(state_);
   const ScanDims d = scan_dims(src, gate, indptr);
   auto out = torch::empty_like(src);
   auto last = want_last ? state_like(src, indptr) : no_tensor(src);
+  auto wide = want_wide ? torch::empty(src.sizes(), src.options().dtype(acc_dtype(src))) : no_tensor(src);
   BatchedRows rows = batched_rows(expand_indptr(indptr, src));
   const size_t ws_bytes = tsb_scan_csr_workspace_bytes(d.B, d.E, d.K, d.N, d.width, dtype_enum(src), dtype_enum(gate));
   auto workspace = torch::empty({(int64_t)ws_bytes}, src.options().dtype(torch::kUInt8));
   check_status(tsb_scan_csr(src.data_ptr(), gate.data_ptr(), rows.ptr(), opt_ptr(state), out.data_ptr(), want_last ? last.data_ptr() : nullptr,
-                            d.B, d.E, d.K, d.N, d.width, rows.batch_stride, dtype_enum(src), dtype_enum(gate), workspace.data_ptr(), ws_bytes,
+                            want_wide ? wide.data_ptr() : nullptr, d.B, d.E, d.K, d.N, d.width, rows.batch_stride, dtype_enum(src), dtype_enum(gate), workspace.data_ptr(), ws_bytes,
                             current_stream()),
                "tsb_scan_csr");
-  return std::make_tuple(out, last);
+  return std::make_tuple(out, last, wide);
 }
 
 // (grad_src, grad_gate, grad_state); the last two are placeholders where they are not wanted
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> scan_bw_impl(std::optional<torch::Tensor> grad_out_, std::optional<torch::Tensor> grad_last_,
-                                                                     torch::Tensor gate_, torch::Tensor out_, torch::Tensor indptr,
-                                                                     std::optional<torch::Tensor> state_, bool want_gate, bool want_state) {
+                                                                     torch::Tensor gate_, torch::Tensor out_, std::optional<torch::Tensor> wide_,
+                                                                     torch::Tensor indptr, std::optional<torch::Tensor> state_, bool want_gate,
+                                                                     bool want_state) {
   c10::cuda::CUDAGuard guard(out_.device());
   auto gate = gate_.contiguous(), out = out_.contiguous();
+  auto wide = opt_contiguous(wide_);
   auto grad_out = opt_contiguous(grad_out_), grad_last = opt_contiguous(grad_last_), state = opt_contiguous(state_);
   const ScanDims d = scan_dims(out, gate, indptr);
   auto grad_src = torch::empty_like(out);
@@ -68,7 +71,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> scan_bw_impl(std::option
   BatchedRows rows = batched_rows(expand_indptr(indptr, out));
   const size_t ws_bytes = tsb_scan_csr_backward_workspace_bytes(d.B, d.E, d.K, d.N, d.width, dtype_enum(out), dtype_enum(gate));
   auto workspace = torch::empty({(int64_t)ws_bytes}, out.options().dtype(torch::kUInt8));
-  check_status(tsb_scan_csr_backward(opt_ptr(grad_out), opt_ptr(grad_last), gate.data_ptr(), out.data_ptr(), rows.ptr(), opt_ptr(state),
+  check_status(tsb_scan_csr_backward(opt_ptr(grad_out), opt_ptr(grad_last), gate.data_ptr(),
+                                     wide.has_value() ? wide.value().data_ptr() : out.data_ptr(), rows.ptr(), opt_ptr(state),
                                      grad_src.data_ptr(), want_gate ? grad_gate.data_ptr() : nullptr, want_state ? grad_state.data_ptr() : nullptr,
                                      d.B, d.E, d.K, d.N, d.width, rows.batch_stride, dtype_enum(out), dtype_enum(gate), workspace.data_ptr(), ws_bytes,
                                      current_stream()),
@@ -78,27 +82,28 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> scan_bw_impl(std::option
 
 class ScanCSR : public torch::autograd::Function<ScanCSR> {
 public:
-  static variable_list forward(AutogradContext *ctx, Variable src, Variable gate, Variable indptr, std::optional<Variable> state, bool want_last) {
-    static auto op = internal_op<std::tuple<torch::Tensor, torch::Tensor>(torch::Tensor, torch::Tensor, torch::Tensor, std::optional<torch::Tensor>, bool)>(
-        "torch_scatter::_scan_csr_fw");
-    auto r = op.call(src, gate, indptr, state, want_last);
+  static variable_list forward(AutogradContext *ctx, Variable src, Variable gate, Variable indptr, std::optional<Variable> state, bool want_last,
+                               bool want_wide) {
+    static auto op = internal_op<std::tuple<torch::Tensor, torch::Tensor, torch::Tensor>(torch::Tensor, torch::Tensor, torch::Tensor,
+                                                                                         std::optional<torch::Tensor>, bool, bool)>("torch_scatter::_scan_csr_fw");
+    auto r = op.call(src, gate, indptr, state, want_last, want_wide);
     ctx->saved_data["want_gate"] = gate.requires_grad();
     ctx->saved_data["want_state"] = state.has_value() && state.value().requires_grad();
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({gate, std::get<0>(r), indptr, state.has_value() ? state.value() : Variable()});
+    ctx->save_for_backward({gate, std::get<0>(r), indptr, state.has_value() ? state.value() : Variable(), want_wide ? std::get<2>(r) : Variable()});
     if (want_last) return {std::get<0>(r), std::get<1>(r)};
     return {std::get<0>(r)};
   }
   static variable_list backward(AutogradContext *ctx, variable_list grad_outs) {
     static auto op = internal_op<std::tuple<torch::Tensor, torch::Tensor, torch::Tensor>(std::optional<torch::Tensor>, std::optional<torch::Tensor>,
-                                                                                         torch::Tensor, torch::Tensor, torch::Tensor,
+                                                                                         torch::Tensor, torch::Tensor, std::optional<torch::Tensor>, torch::Tensor,
                                                                                          std::optional<torch::Tensor>, bool, bool)>("torch_scatter::_scan_csr_bw");
     auto saved = ctx->get_saved_variables();
     auto gate = saved[0], out = saved[1], indptr = saved[2], state = saved[3];
     const bool want_gate = ctx->saved_data["want_gate"].toBool(), want_state = ctx->saved_data["want_state"].toBool();
     const auto grad_last = grad_outs.size() > 1 ? some_if_defined(grad_outs[1]) : std::nullopt;
-    auto r = op.call(some_if_defined(grad_outs[0]), grad_last, gate, out, indptr, some_if_defined(state), want_gate, want_state);
-    return first_order({std::get<0>(r), want_gate ? std::get<1>(r) : Variable(), Variable(), want_state ? std::get<2>(r) : Variable(), Variable()},
+    auto r = op.call(some_if_defined(grad_outs[0]), grad_last, gate, out, some_if_defined(saved[4]), indptr, some_if_defined(state), want_gate, want_state);
+    return first_order({std::get<0>(r), want_gate ? std::get<1>(r) : Variable(), Variable(), want_state ? std::get<2>(r) : Variable(), Variable(), Variable()},
                        {grad_outs[0], grad_last.has_value() ? grad_last.value() : Variable(), gate, out, state});
   }
 };
@@ -144,7 +149,9 @@ variable_list scan(const char *name, torch::Tensor src, torch::Tensor gate, torc
     for (int64_t i = 0; i < src.dim(); i++)
       TORCH_CHECK(s.size(i) == (i == dim ? indptr.size(-1) - 1 : src.size(i)), name, ": state must have src's shape with one row for each segment");
   }
-  return ScanCSR::apply(src, gate, indptr, state, want_last);
+  // with a gate wider than the data the gradient of the gate needs h unrounded (see the kernel)
+  const bool want_wide = gate.scalar_type() != src.scalar_type() && gate.requires_grad() && at::GradMode::is_enabled();
+  return ScanCSR::apply(src, gate, indptr, state, want_last, want_wide);
 }
 
 torch::Tensor scan_csr(torch::Tensor src, torch::Tensor gate, torch::Tensor indptr, std::optional<torch::Tensor> state) {
@@ -199,8 +206,8 @@ TORCH_LIBRARY_FRAGMENT(torch_scatter, m) {
   m.def("scan_csr", &tsb_ops::scan_csr);
   m.def("scan_csr_state", &tsb_ops::scan_csr_state);
   m.def("scan_step(Tensor src, Tensor gate, Tensor(a!) state) -> Tensor", &tsb_ops::scan_step);
-  m.def("_scan_csr_fw(Tensor src, Tensor gate, Tensor indptr, Tensor? state, bool want_last) -> (Tensor, Tensor)");
-  m.def("_scan_csr_bw(Tensor? grad_out, Tensor? grad_last, Tensor gate, Tensor out, Tensor indptr, Tensor? state, bool want_gate, "
+  m.def("_scan_csr_fw(Tensor src, Tensor gate, Tensor indptr, Tensor? state, bool want_last, bool want_wide) -> (Tensor, Tensor, Tensor)");
+  m.def("_scan_csr_bw(Tensor? grad_out, Tensor? grad_last, Tensor gate, Tensor out, Tensor? wide, Tensor indptr, Tensor? state, bool want_gate, "
         "bool want_state) -> (Tensor, Tensor, Tensor)");
   m.def("_scan_step(Tensor src, Tensor gate, Tensor(a!) state) -> Tensor");
 }

@@ -295,10 +295,12 @@ def test_scan(kind, heads, width, states, dtype, gdtype):
         grads = torch.autograd.grad(out, (xs, xg), grad.cuda())
     assert grads[0].dtype == dtype and grads[1].dtype == gdtype
     ref.assert_within(grads[0].reshape(E, K), dh, dbound + ref.last_rounding(dh, dtype), 'grad_src')
-    # grad_gate = sum dh * before; `before` is the rounded output, its first row of a segment the state itself
+    # grad_gate = sum dh * before; `before` is the rounded output (unrounded where the gate is wider than the data), its
+    # first row of a segment the state itself
+    rounded = ref.last_rounding(before, dtype) if gdtype == dtype else 0
     first = torch.zeros(E, 1)
     first[[e for e, n in zip(ends, lens) if n]] = 1
-    err = dh.abs() * (torch.roll(bound, 1, 0) + ref.last_rounding(before, dtype)) * (1 - first) + dbound * before.abs() + u * dg.abs()
+    err = dh.abs() * (torch.roll(bound, 1, 0) + rounded) * (1 - first) + dbound * before.abs() + u * dg.abs()
     dg3, err3 = dg.reshape(E, heads, width), err.reshape(E, heads, width)
     want = dg3.sum(-1, keepdim=True)
     err3 = err3.sum(-1, keepdim=True) + u * width * dg3.abs().sum(-1, keepdim=True) + ref.last_rounding(want, gdtype)
