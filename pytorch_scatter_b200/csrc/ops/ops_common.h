@@ -133,6 +133,13 @@ inline void check_float_dtype(const torch::Tensor &t, const char *name) {
   TORCH_CHECK(s == at::ScalarType::Float || s == at::ScalarType::Double || s == at::ScalarType::Half || s == at::ScalarType::BFloat16,
               name, " must be a float32, float64, float16 or bfloat16 tensor, got ", s);
 }
+// No gradient can be asked for: the operator is called without an autograd node around it (2 us of the host's time).
+inline bool no_grad_for(std::initializer_list<torch::Tensor> ts) {
+  if (!at::GradMode::is_enabled()) return true;
+  for (auto &t : ts)
+    if (t.defined() && t.requires_grad()) return false;
+  return true;
+}
 inline const void *opt_ptr(const std::optional<torch::Tensor> &t) { return t.has_value() ? t.value().data_ptr() : nullptr; }
 inline std::optional<torch::Tensor> opt_contiguous(const std::optional<torch::Tensor> &t) {
   return t.has_value() ? std::optional<torch::Tensor>(t.value().contiguous()) : std::nullopt;

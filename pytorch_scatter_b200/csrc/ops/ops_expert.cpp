@@ -38,11 +38,15 @@ torch::Tensor topk_bw_impl(torch::Tensor grad_, torch::Tensor logits_, torch::Te
   return out;
 }
 
+std::tuple<torch::Tensor, torch::Tensor> topk_fw(const torch::Tensor &logits, int64_t k, bool normalize) {
+  static auto op = internal_op<std::tuple<torch::Tensor, torch::Tensor>(torch::Tensor, int64_t, bool)>("torch_scatter::_expert_topk_fw");
+  return op.call(logits, k, normalize);
+}
+
 class ExpertTopk : public torch::autograd::Function<ExpertTopk> {
 public:
   static variable_list forward(AutogradContext *ctx, Variable logits, int64_t k, bool normalize) {
-    static auto op = internal_op<std::tuple<torch::Tensor, torch::Tensor>(torch::Tensor, int64_t, bool)>("torch_scatter::_expert_topk_fw");
-    auto r = op.call(logits, k, normalize);
+    auto r = topk_fw(logits, k, normalize);
     ctx->saved_data["normalize"] = normalize;
     ctx->save_for_backward({logits, std::get<0>(r), std::get<1>(r)});
     ctx->mark_non_differentiable({std::get<1>(r)});
@@ -64,6 +68,7 @@ std::tuple<torch::Tensor, torch::Tensor> expert_topk(torch::Tensor logits, int64
   TORCH_CHECK(logits.dim() >= 1, "expert_topk: logits must have a last dimension of experts");
   TORCH_CHECK(logits.size(-1) >= 1 && logits.size(-1) <= 1024, "expert_topk: 1 to 1024 experts are supported, got ", std::to_string(logits.size(-1)));
   TORCH_CHECK(k >= 1 && k <= logits.size(-1), "expert_topk: k must be between 1 and the number of experts (", std::to_string(logits.size(-1)), "), got ", std::to_string(k));
+  if (no_grad_for({logits})) return topk_fw(logits, k, normalize);
   auto r = ExpertTopk::apply(logits, k, normalize);
   return std::make_tuple(r[0], r[1]);
 }
@@ -199,12 +204,14 @@ torch::Tensor expert_dispatch(torch::Tensor src, torch::Tensor slot, torch::Tens
   TORCH_CHECK(src.dim() >= lead, "expert_dispatch: src must begin with slot's dimensions of tokens");
   for (int64_t i = 0; i < lead; i++)
     TORCH_CHECK(src.size(i) == slot.size(i), "expert_dispatch: src must begin with slot's dimensions of tokens");
+  if (no_grad_for({src, weight.value_or(torch::Tensor())})) return std::get<0>(spread(src, slot, indptr, weight, std::nullopt));
   return ExpertRows<true>::apply(src, slot, indptr, weight)[0];
 }
 
 torch::Tensor expert_combine(torch::Tensor rows, torch::Tensor slot, torch::Tensor indptr, std::optional<torch::Tensor> weight) {
   check_plan("expert_combine", rows, slot, indptr, weight);
   TORCH_CHECK(rows.dim() >= 1 && rows.size(0) == slot.numel(), "expert_combine: rows must have one row for each entry of slot (", std::to_string(slot.numel()), ")");
+  if (no_grad_for({rows, weight.value_or(torch::Tensor())})) return std::get<0>(fold(rows, slot, weight, std::nullopt));
   return ExpertRows<false>::apply(rows, slot, indptr, weight)[0];
 }
 

@@ -80,13 +80,18 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> scan_bw_impl(std::option
   return std::make_tuple(grad_src, grad_gate, grad_state);
 }
 
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> scan_fw(const torch::Tensor &src, const torch::Tensor &gate, const torch::Tensor &indptr,
+                                                                const std::optional<torch::Tensor> &state, bool want_last, bool want_wide) {
+  static auto op = internal_op<std::tuple<torch::Tensor, torch::Tensor, torch::Tensor>(torch::Tensor, torch::Tensor, torch::Tensor,
+                                                                                       std::optional<torch::Tensor>, bool, bool)>("torch_scatter::_scan_csr_fw");
+  return op.call(src, gate, indptr, state, want_last, want_wide);
+}
+
 class ScanCSR : public torch::autograd::Function<ScanCSR> {
 public:
   static variable_list forward(AutogradContext *ctx, Variable src, Variable gate, Variable indptr, std::optional<Variable> state, bool want_last,
                                bool want_wide) {
-    static auto op = internal_op<std::tuple<torch::Tensor, torch::Tensor, torch::Tensor>(torch::Tensor, torch::Tensor, torch::Tensor,
-                                                                                         std::optional<torch::Tensor>, bool, bool)>("torch_scatter::_scan_csr_fw");
-    auto r = op.call(src, gate, indptr, state, want_last, want_wide);
+    auto r = scan_fw(src, gate, indptr, state, want_last, want_wide);
     ctx->saved_data["want_gate"] = gate.requires_grad();
     ctx->saved_data["want_state"] = state.has_value() && state.value().requires_grad();
     ctx->set_materialize_grads(false);
@@ -149,8 +154,12 @@ variable_list scan(const char *name, torch::Tensor src, torch::Tensor gate, torc
     for (int64_t i = 0; i < src.dim(); i++)
       TORCH_CHECK(s.size(i) == (i == dim ? indptr.size(-1) - 1 : src.size(i)), name, ": state must have src's shape with one row for each segment");
   }
+  if (no_grad_for({src, gate, state.value_or(torch::Tensor())})) {
+    auto r = scan_fw(src, gate, indptr, state, want_last, false);
+    return {std::get<0>(r), std::get<1>(r)};
+  }
   // with a gate wider than the data the gradient of the gate needs h unrounded (see the kernel)
-  const bool want_wide = gate.scalar_type() != src.scalar_type() && gate.requires_grad() && at::GradMode::is_enabled();
+  const bool want_wide = gate.scalar_type() != src.scalar_type() && gate.requires_grad();
   return ScanCSR::apply(src, gate, indptr, state, want_last, want_wide);
 }
 

@@ -383,6 +383,52 @@ def test_scan_sequences_do_not_leak():
     assert bool(gs[~touched].isfinite().all()) and bool(gg[~touched].isfinite().all())
 
 
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+@pytest.mark.parametrize('offset', [1, 2, 3, 4])
+@pytest.mark.parametrize('K', [24, 7])
+def test_scan_data_off_a_boundary(dtype, offset, K):
+    """Inputs that begin anywhere in their storage, the first and the last value of it included; a gate wider than the data."""
+    gen = torch.Generator().manual_seed(offset)
+    E, ends = 300, [0, 120, 300]
+    src, grad = rand(gen, E, K, dtype=dtype), rand(gen, E, K, dtype=dtype)
+    gate = torch.sigmoid(rand(gen, E, K) + 2)
+
+    def off(t):
+        buf = torch.empty(t.numel() + offset, dtype=t.dtype, device='cuda')
+        return buf[offset:].view(t.shape).copy_(t)
+
+    for g in ([gate] if dtype == F32 else [gate, gate.to(dtype)]):
+        h, before, _, mass, way = ref.scan(src.double(), g.double(), ends, None)
+        dh, dg, _, dmass, dway, _, _ = ref.scan_backward(grad.double(), None, g.double(), before, ends)
+        u = ref.unit(dtype)
+        bound, dbound = u * (4 * way + 32 * mass), u * (4 * dway + 32 * dmass)
+        xs, xg = off(src).requires_grad_(), off(g).requires_grad_()
+        out = ts.scan_csr(xs, xg, torch.tensor(ends, device='cuda'))
+        gs, gg = torch.autograd.grad(out, (xs, xg), off(grad))
+        ref.assert_within(out, h, bound + ref.last_rounding(h, dtype), 'out')
+        ref.assert_within(gs, dh, dbound + ref.last_rounding(dh, dtype), 'grad_src')
+        rounded = ref.last_rounding(before, dtype) if g.dtype == dtype else 0
+        err = dh.abs() * (torch.roll(bound, 1, 0) + rounded) + dbound * before.abs() + u * dg.abs()
+        ref.assert_within(gg, dg, err + ref.last_rounding(dg, g.dtype), 'grad_gate')
+
+
+def test_scan_many_empty_segments_and_a_long_stream():
+    """Runs of empty segments around and inside tiles, and rows by the hundred thousand (several rounds of a cluster)."""
+    gen = torch.Generator().manual_seed(12)
+    lens = torch.randint(0, 3, (4000,), generator=gen) * (torch.rand(4000, generator=gen) < 0.05)
+    lens[1000], lens[3000] = 70000, 40000
+    ends = torch.cat([torch.zeros(1, dtype=torch.long), lens.cumsum(0)])
+    E = int(ends[-1])
+    src, gate = torch.ones(E, 8, device='cuda'), torch.full((E, 8), 0.5, device='cuda')
+    out, last = ts.scan_csr_state(src, gate, ends.cuda(), torch.full((4000, 8), 2.0, device='cuda'))
+    # a fixed point: 0.5 * 2 + 1 = 2 exactly, whatever the segments are
+    assert bool((out == 2).all()) and bool((last == 2).all())
+    out = ts.scan_csr(src, torch.ones_like(gate), ends.cuda())
+    # counts of the rows of each segment: whole numbers below 2^24, exact in any order
+    row = torch.arange(E) - torch.repeat_interleave(ends[:-1], lens) + 1
+    assert torch.equal(out.cpu(), row.float().unsqueeze(1).expand(E, 8))
+
+
 def test_scan_empty_shapes():
     z = torch.zeros
     p = torch.tensor([0, 0, 0], device='cuda')
@@ -415,6 +461,15 @@ def test_step(n, heads, width, dtype, gdtype):
     assert not bool(pool[:, 0].any())
     full, last = ts.scan_csr_state(src.cuda(), gate.cuda(), torch.arange(n + 1, device='cuda'), state.cuda())
     assert torch.equal(last, s) and torch.equal(full, out)
+
+
+def test_step_compiles():
+    state = torch.randn(4, 6, device='cuda')
+    x, g = torch.randn(4, 6, device='cuda'), torch.rand(4, 6, device='cuda')
+    want_state = g * state + x
+    with torch.no_grad():
+        out = torch.compile(lambda a, b, s: ts.scan_step(a, b, s) * 2, fullgraph=True)(x, g, state)
+    assert torch.allclose(state, want_state, rtol=1e-6, atol=1e-6) and torch.allclose(out, 2 * want_state, rtol=1e-6, atol=1e-6)
 
 
 def test_step_marks_the_state_as_changed():
