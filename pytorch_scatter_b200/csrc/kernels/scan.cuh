@@ -81,15 +81,119 @@ template <typename T, int VEC> struct Slot {
   }
 };
 
-template <typename A, int VEC> __device__ __forceinline__ void load_acc(A (&v)[VEC], const void *base, int64_t at) {
+// Rows that begin anywhere (60000 x 333 fp16 in 3001 segments, forward / backward: 126 / 187 us; one channel to a thread
+// instead: 191 / 369): the lanes of a row share its aligned 16-byte chunks, n of them to a lane and one more, and a
+// lane shifts its values out of its own and the next one (the lanes of a row are lanes of one warp).
+template <typename X, int VEC> struct Ragged {
+  static constexpr int n = (int)sizeof(X) * VEC / 16;
+  static __device__ __forceinline__ void copy_chunk(char *dst, uintptr_t src, bool edge, const X *lo, const X *hi) {
+    if (!edge || (src >= reinterpret_cast<uintptr_t>(lo) && src + 16 <= reinterpret_cast<uintptr_t>(hi))) {
+      const unsigned to = (unsigned)__cvta_generic_to_shared(dst);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
+    } else {  // over the array's ends
+      const X *p = reinterpret_cast<const X *>(src);
+#pragma unroll
+      for (int i = 0; i < 16 / (int)sizeof(X); ++i)
+        if (p + i >= lo && p + i < hi) reinterpret_cast<X *>(dst)[i] = p[i];
+    }
+  }
+  // p: the row's first value of the tile, of `bytes` that belong to the row
+  static __device__ __forceinline__ void copy(char *row, const X *p, int col, int lx, int bytes, bool edge, const X *lo, const X *hi) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p), base = at & ~(uintptr_t)15;
+    const int end = (int)(at & 15) + bytes;
+#pragma unroll
+    for (int i = 0; i < n; ++i)
+      if ((col * n + i) * 16 < end) copy_chunk(row + (col * n + i) * 16, base + (col * n + i) * 16, edge, lo, hi);
+    if (col == lx - 1 && lx * n * 16 < end) copy_chunk(row + lx * n * 16, base + lx * n * 16, edge, lo, hi);
+  }
+  // off: bytes between the aligned chunk and the row's first value
+  static __device__ __forceinline__ Pack<X, VEC> get(const char *row, int col, int off) {
+    unsigned w[4 * n + 4];
+#pragma unroll
+    for (int i = 0; i <= n; ++i) {
+      const uint4 q = *reinterpret_cast<const uint4 *>(row + (col * n + i) * 16);
+      w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+    }
+#pragma unroll
+    for (int i = 0; i < 4 * n + 2; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+    if constexpr (sizeof(X) <= 4) {
+#pragma unroll
+      for (int i = 0; i < 4 * n + 1; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+    }
+    if constexpr (sizeof(X) <= 2) {
+#pragma unroll
+      for (int i = 0; i < 4 * n; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], off & 2 ? 16 : 0);
+    }
+    Pack<X, VEC> r;
+    unsigned *out = reinterpret_cast<unsigned *>(&r);
+#pragma unroll
+    for (int i = 0; i < 4 * n; ++i) out[i] = w[i];
+    return r;
+  }
+  // The way back, all lanes of a row together (`lanes`): a lane writes its aligned chunks, whose first values are the last
+  // of the lane before.  p: the row's first value of the tile.  The row's ends are written value by value.
+  static __device__ __forceinline__ void store(X *p, const Pack<X, VEC> &v, int col, int lx, int bytes, unsigned lanes) {
+    constexpr int V = 16 / (int)sizeof(X);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const int off = (int)(at & 15), end = off + bytes;
+    X *base = reinterpret_cast<X *>(at & ~(uintptr_t)15);
+    const unsigned *own = reinterpret_cast<const unsigned *>(&v);
+    unsigned w[4 * n + 4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __shfl_up_sync(lanes, own[4 * n - 4 + i], 1);
+#pragma unroll
+    for (int i = 0; i < 4 * n; ++i) w[4 + i] = own[i];
+    // skip 16 - off bytes of these; with off = 0 that is all of the neighbour's
+    if (off == 0) {
+#pragma unroll
+      for (int i = 0; i < 4 * n; ++i) w[i] = w[i + 4];
+    } else {
+      const int skip = 16 - off;
+#pragma unroll
+      for (int i = 0; i < 4 * n + 2; ++i) w[i] = skip & 8 ? w[i + 2] : w[i];
+      if constexpr (sizeof(X) <= 4) {
+#pragma unroll
+        for (int i = 0; i < 4 * n + 1; ++i) w[i] = skip & 4 ? w[i + 1] : w[i];
+      }
+      if constexpr (sizeof(X) <= 2) {
+#pragma unroll
+        for (int i = 0; i < 4 * n; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], skip & 2 ? 16 : 0);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < n; ++c) {
+      const int first = (col * n + c) * 16;
+      const X *x = reinterpret_cast<const X *>(&w[4 * c]);
+      if (first >= off && first + 16 <= end) {
+        __stcs(reinterpret_cast<uint4 *>(base + first / (int)sizeof(X)), make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int b = first + i * (int)sizeof(X);
+          if (b >= off && b < end) base[b / (int)sizeof(X)] = x[i];
+        }
+      }
+    }
+    if (col == lx - 1 && off > 0) {  // what reaches into the chunk behind the last lane's
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const int b = off + (col * VEC + i) * (int)sizeof(X);
+        if (b >= lx * n * 16 && b < end) base[b / (int)sizeof(X)] = v.v[i];
+      }
+    }
+  }
+};
+
+template <typename A, int VEC> __device__ __forceinline__ void load_acc(A (&v)[VEC], const void *base, int64_t at, int nv) {
   const A *p = static_cast<const A *>(base);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) v[i] = p ? p[at + i] : (A)0;
+  for (int i = 0; i < VEC; ++i) v[i] = p && i < nv ? p[at + i] : (A)0;
 }
-template <typename A, int VEC> __device__ __forceinline__ void store_acc(const A (&v)[VEC], void *base, int64_t at) {
+template <typename A, int VEC> __device__ __forceinline__ void store_acc(const A (&v)[VEC], void *base, int64_t at, int nv) {
   A *p = static_cast<A *>(base);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) p[at + i] = v[i];
+  for (int i = 0; i < VEC; ++i)
+    if (i < nv) p[at + i] = v[i];
 }
 
 // VEC values of one thread to and from shared memory, 16 bytes at a time where there are as many
@@ -240,7 +344,7 @@ __device__ __forceinline__ void send(unsigned addr, unsigned bar, float a, float
 __device__ __forceinline__ void send(unsigned addr, unsigned bar, double a, double b) {
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f64 [%0], {%1, %2}, [%3];" ::"r"(addr), "d"(a), "d"(b), "r"(bar) : "memory");
 }
-template <typename T, typename G, int VEC, bool SHARED, bool BWD> struct ScanShape {
+template <typename T, typename G, int VEC, bool SHARED, bool BWD, bool RAGGED> struct ScanShape {
   using A = acc_t<T>;
   static constexpr int kGateVec = SHARED ? 1 : VEC;
   // The backward multiplies dh by the h before it.  With a gate of the data's type that is the rounded output: the
@@ -254,32 +358,41 @@ template <typename T, typename G, int VEC, bool SHARED, bool BWD> struct ScanSha
   // Rows of a thread: 42 KB for each of the two stages at most, so that two CTAs fit an SM.  What a tile costs besides its
   // rows, step (2), is then a small part (65536 x 4096 bf16: 291 us with 10 rows and 2 stages, 302 with 7 rows and 3
   // stages, 391 with 5 rows, 2 stages and four CTAs).
-  static constexpr int kRows = 336 / kRowBytes < 16 ? 336 / kRowBytes : 16;
+  static constexpr int kRows = (RAGGED ? 296 : 336) / kRowBytes < 16 ? (RAGGED ? 296 : 336) / kRowBytes : 16;
   static constexpr int kCtas = kRowBytes <= 16 ? 4 : 2;  // of an SM, by the registers
-  static constexpr int kStageBytes = kScanThreads * kRows * kRowBytes;
+  // of the two stages; ragged rows have one more chunk in each array
+  static __host__ __device__ int stage_bytes(int lx) {
+    return kScanThreads * kRows * kRowBytes + (RAGGED ? kScanThreads / lx * kRows * 16 * (BWD ? 3 : 2) : 0);
+  }
   static constexpr int kMaps = kScanThreads * VEC + 128;      // [ty][C], see `skew`
   static constexpr int kMapBytes = 2 * kMaps * (int)sizeof(A);
   static size_t bytes(int lx, int cluster) {
     const size_t C = (size_t)lx * VEC, L = (size_t)(kScanThreads / lx) * kRows;
-    return (size_t)kStages * kStageBytes + kMapBytes + (cluster > 1 ? sizeof(A) * C * 4 * cluster : 0) + sizeof(int) * kMarkStages * L;
+    return (size_t)kStages * stage_bytes(lx) + kMapBytes + (cluster > 1 ? sizeof(A) * C * 4 * cluster : 0) + sizeof(int) * kMarkStages * L;
   }
 };
 
-template <typename T, typename G, int VEC, bool SHARED, bool BWD>
-__global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED, BWD>::kCtas) scan_kernel(ScanParams p) {
-  using S = ScanShape<T, G, VEC, SHARED, BWD>;
+template <typename T, typename G, int VEC, bool SHARED, bool BWD, bool RAGGED>
+__global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED, BWD, RAGGED>::kCtas) scan_kernel(ScanParams p) {
+  using S = ScanShape<T, G, VEC, SHARED, BWD, RAGGED>;
   using SrcSlot = typename S::SrcSlot;
   using GateSlot = typename S::GateSlot;
   using FwdSlot = typename S::FwdSlot;
   using F = typename S::F;
   using A = acc_t<T>;
   constexpr int R = S::kRows;
-  constexpr int kSrcRow = kScanThreads * SrcSlot::kBytes, kGateRow = kScanThreads * GateSlot::kBytes,
-                kFwdRow = kScanThreads * FwdSlot::kBytes;
+  // A ragged row is a few hundred instructions: unrolled, the loops over a thread's rows do not fit the instruction cache
+  // (60000 x 333 fp16 in 3001 segments: 243 us, most of it waiting for instructions, against 126).
+  constexpr int kUnroll = RAGGED ? 1 : R;
+
 
   const int tid = threadIdx.x;
   const int lx = 1 << p.lx_log2, C = lx * VEC, L = (kScanThreads >> p.lx_log2) * R;
   const int col = tid & (lx - 1), ty = tid >> p.lx_log2;
+  // shared memory from a thread's row to its next one, and of a ragged row (one more chunk than its lanes hold)
+  const int ragged_row = RAGGED ? (kScanThreads >> p.lx_log2) * 16 : 0;
+  const int kSrcRow = kScanThreads * SrcSlot::kBytes + ragged_row, kGateRow = kScanThreads * GateSlot::kBytes + ragged_row,
+            kFwdRow = kScanThreads * FwdSlot::kBytes + ragged_row;
   const int cs = p.cluster, rank = (int)(blockIdx.x % cs);
   int64_t id = blockIdx.x / cs;
   const int64_t kt = id % p.tiles_k;
@@ -293,7 +406,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
   const int64_t step = (int64_t)cs * L;
 
   extern __shared__ __align__(128) char smem[];
-  A *s_a = reinterpret_cast<A *>(smem + (size_t)kStages * S::kStageBytes);  // maps of the threads [ty][C]; then the values
+  A *s_a = reinterpret_cast<A *>(smem + (size_t)kStages * S::stage_bytes(lx));  // maps of the threads [ty][C]; then the values
   A *s_b = s_a + S::kMaps;                                         // that reach them, in place of A
   A *s_total = s_b + S::kMaps;                           // maps of the cluster's CTAs [2][cs][C][A, B]
   int *s_marks = reinterpret_cast<int *>(s_total + (cs > 1 ? 4 * cs * C : 0));  // [stage][L]
@@ -363,6 +476,8 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
 
   const int64_t c0 = kt * C + (int64_t)col * VEC;   // this thread's first channel
   const bool live = c0 < p.K;
+  const int nv = RAGGED ? (int)(p.K - c0 < VEC ? p.K - c0 : VEC) : VEC;  // channels of this thread that there are
+  const int tile_c = (int)(p.K - kt * C < C ? p.K - kt * C : C);           // and of the tile
   const int64_t gates = p.K / p.width, g0 = SHARED ? c0 / p.width : c0;
   const int64_t dk = BWD ? -p.K : p.K, dgates = BWD ? -gates : gates;  // from a row to the next one on the way
   const int64_t srow = b * p.N;                     // first row of this batch in the state arrays
@@ -372,9 +487,9 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
   const G *gate_lo = static_cast<const G *>(p.gate), *gate_hi = gate_lo + p.B * p.E * gates;
 
   // this thread's slots [stage][row][thread], and its pointers to the next tile to load and to the tile at work
-  char *s_src = smem + tid * SrcSlot::kBytes;
-  char *s_fwd = smem + kStages * R * kSrcRow + tid * FwdSlot::kBytes;
-  char *s_gate = smem + kStages * R * (kSrcRow + (BWD ? kFwdRow : 0)) + tid * GateSlot::kBytes;
+  char *s_src = smem + (RAGGED ? ty * (lx * SrcSlot::kBytes + 16) : tid * SrcSlot::kBytes);
+  char *s_fwd = smem + kStages * R * kSrcRow + (RAGGED ? ty * (lx * FwdSlot::kBytes + 16) : tid * FwdSlot::kBytes);
+  char *s_gate = smem + kStages * R * (kSrcRow + (BWD ? kFwdRow : 0)) + (RAGGED ? ty * (lx * GateSlot::kBytes + 16) : tid * GateSlot::kBytes);
   int64_t tile = (int64_t)rank * L;                 // position of the CTA's tile
   int64_t ahead = tile + ty * R;                    // position of the thread's next rows to load
   const int64_t at = b * p.E + row_of(ahead);
@@ -390,28 +505,40 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
   const bool part_sums = SHARED && sums != gates;
   A *op = static_cast<A *>(p.partial) + (part_sums && want_gate ? at * sums + c0 / ((int64_t)VEC * sum_lanes) : 0);
   const int64_t tile_k = step * dk, tile_gates = step * dgates;
-  // which half of its word a row's value is in (2-byte slots only)
-  const int kodd = (int)(p.K & 1), godd = (int)(gates & 1);
-  int xhalf = SrcSlot::half(lsrc), fhalf = FwdSlot::half(lfwd), ghalf = GateSlot::half(lgate);
-  const int xturn = (int)(tile_k & 1), gturn = (int)(tile_gates & 1);
+  // Where a row's values are: the half of its word (2-byte slots), or the bytes between the aligned chunk and the row's
+  // first value (ragged rows).  From row to row and from tile to tile this moves by the row length.
+  const int kcol = RAGGED ? col * VEC : 0;
+  const auto where = [&](auto *q, int slot_half) { return RAGGED ? (int)(reinterpret_cast<uintptr_t>(q - kcol) & 15) : slot_half; };
+  const auto moved = [&](int from, int64_t rows, int64_t row_len, int size) {
+    return RAGGED ? (int)(from + rows * row_len * size) & 15 : (int)(from + rows * row_len) & 1;
+  };
+  int xat = where(lsrc, SrcSlot::half(lsrc)), fat = where(lfwd, FwdSlot::half(lfwd)), gat = where(lgate, GateSlot::half(lgate));
 
+  const int64_t margin = RAGGED ? 1 + 16 / (p.K * (int64_t)(sizeof(T) < sizeof(G) ? sizeof(T) : sizeof(G))) : 0;  // rows in 16 bytes
   const auto load_rows = [&](int stage) {
     const int64_t left = len - ahead;
-    if (live && left > 0) {
+    if (RAGGED) __syncwarp();  // the lanes of a row have read each other's chunks of this stage
+    if ((live || (RAGGED && (col - 1) * VEC < tile_c)) && left > 0) {  // (a ragged row may end in the chunk of the lane behind)
       const T *xs = lsrc;
       const F *fs = lfwd;
       const G *gs = lgate;
       char *xd = s_src + stage * (R * kSrcRow), *fd = s_fwd + stage * (R * kFwdRow), *gd = s_gate + stage * (R * kGateRow);
       const int n = left < R ? (int)left : R;
-      // only the first and the last row of the whole array hold words that reach over its ends
+      // only the first and the last rows of the whole array hold words or chunks that reach over its ends
       const int64_t row = b * p.E + row_of(ahead);
-      const bool edge = BWD ? row <= R || row >= p.B * p.E - 1 : row <= 0 || row + R >= p.B * p.E;
-#pragma unroll
+      const bool edge = BWD ? row <= R + margin || row >= p.B * p.E - 1 - margin : row <= margin || row + R >= p.B * p.E - margin;
+#pragma unroll kUnroll
       for (int r = 0; r < R; ++r) {
         if (r < n) {
+          if constexpr (RAGGED) {
+            if (have_src) Ragged<T, VEC>::copy(xd + r * kSrcRow, xs - kcol, col, lx, tile_c * (int)sizeof(T), edge, src_lo, src_hi);
+            Ragged<G, VEC>::copy(gd + r * kGateRow, gs - kcol, col, lx, tile_c * (int)sizeof(G), edge, gate_lo, gate_hi);
+            if (BWD && want_gate && fs - kcol >= fwd_lo) Ragged<F, VEC>::copy(fd + r * kFwdRow, fs - kcol, col, lx, tile_c * (int)sizeof(F), edge, fwd_lo, fwd_hi);
+          } else {
           if (have_src) SrcSlot::copy(xd + r * kSrcRow, xs, edge, src_lo, src_hi);
           GateSlot::copy(gd + r * kGateRow, gs, edge, gate_lo, gate_hi);
           if (BWD && want_gate && fs >= fwd_lo) FwdSlot::copy(fd + r * kFwdRow, fs, edge, fwd_lo, fwd_hi);  // (row 0 has none before it)
+          }
         }
         xs += dk;
         fs += dk;
@@ -447,14 +574,25 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
     }
     const char *xs = s_src + stage * (R * kSrcRow), *gs = s_gate + stage * (R * kGateRow);
     [[maybe_unused]] const char *fs = s_fwd + stage * (R * kFwdRow);
+    const unsigned rowmask = lx == 32 ? kFullMask : ((1u << lx) - 1u) << ((tid & 31) & ~(lx - 1));  // the lanes of this row
+    const auto store_row = [&](auto *to, const auto &q) {
+      using X = std::remove_pointer_t<decltype(to)>;
+      if constexpr (RAGGED) Ragged<X, VEC>::store(to - kcol, q, col, lx, tile_c * (int)sizeof(X), rowmask);
+      else if (live) st_stream<X, VEC>(to, q);
+    };
     const auto read_row = [&](A (&x)[VEC], A (&g)[VEC], int r) {
-      widen<T, VEC>(x, SrcSlot::get(xs + r * kSrcRow, (xhalf + r * kodd) & 1));
+      if constexpr (RAGGED) {
+        widen<T, VEC>(x, Ragged<T, VEC>::get(xs + r * kSrcRow, col, moved(xat, r, dk, sizeof(T))));
+        widen<G, VEC>(g, Ragged<G, VEC>::get(gs + r * kGateRow, col, moved(gat, r, dgates, sizeof(G))));
+        return;
+      }
+      widen<T, VEC>(x, SrcSlot::get(xs + r * kSrcRow, moved(xat, r, dk, 1)));
       if constexpr (SHARED) {
-        const A one = to_acc<G>(GateSlot::get(gs + r * kGateRow, (ghalf + r * godd) & 1).v[0]);
+        const A one = to_acc<G>(GateSlot::get(gs + r * kGateRow, moved(gat, r, dgates, 1)).v[0]);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) g[v] = one;
       } else {
-        widen<G, VEC>(g, GateSlot::get(gs + r * kGateRow, (ghalf + r * godd) & 1));
+        widen<G, VEC>(g, GateSlot::get(gs + r * kGateRow, moved(gat, r, dgates, 1)));
       }
     };
 
@@ -465,7 +603,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
 #pragma unroll
       for (int v = 0; v < VEC; ++v) { ma[v] = 1; mb[v] = 0; }
       int reset = 0;
-#pragma unroll
+#pragma unroll kUnroll
       for (int r = 0; r < R; ++r) {
         if constexpr (MARKED) {
           const int m = mark[r];
@@ -475,7 +613,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
 #pragma unroll
             for (int v = 0; v < VEC; ++v) mb[v] = 0;
             if (m & kDead) continue;
-            if (live) load_acc<A, VEC>(mb, p.state, (srow + (m >> kMarkBits)) * p.K + c0);
+            if (live) load_acc<A, VEC>(mb, p.state, (srow + (m >> kMarkBits)) * p.K + c0, nv);
           }
         }
         A x[VEC], g[VEC];
@@ -574,7 +712,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
     A *wrow = ow;
     G *grow = og;
     A *prow = op;
-#pragma unroll
+#pragma unroll kUnroll
     for (int r = 0; r < R; ++r, orow += dk, wrow += dk, grow += dgates, prow += dsums) {
       int m = 0;
       if constexpr (MARKED) {
@@ -583,7 +721,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
         if (m & (BWD ? kEnd : kStart)) {
 #pragma unroll
           for (int v = 0; v < VEC; ++v) v_[v] = 0;
-          if (live) load_acc<A, VEC>(v_, p.state, (srow + (m >> kMarkBits)) * p.K + c0);
+          if (live) load_acc<A, VEC>(v_, p.state, (srow + (m >> kMarkBits)) * p.K + c0, nv);
         }
       }
       const bool dead = MARKED && (m & kDead);
@@ -597,11 +735,14 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
           for (int v = 0; v < VEC; ++v) v_[v] = 0;
         }
         round_pack(o, v_);
+        store_row(orow, o);
         if (live) {
-          st_stream<T, VEC>(orow, o);
           if constexpr (!std::is_same<F, T>::value)
-            if (p.wide) store_wide(wrow, v_);
-          if (MARKED && (m & kEnd) && p.last) store_acc<A, VEC>(v_, p.last, (srow + (m >> kMarkBits)) * p.K + c0);
+            if (p.wide) {
+              if (RAGGED) store_acc<A, VEC>(v_, wrow, 0, nv);
+              else store_wide(wrow, v_);
+            }
+          if (MARKED && (m & kEnd) && p.last) store_acc<A, VEC>(v_, p.last, (srow + (m >> kMarkBits)) * p.K + c0, nv);
         }
       } else {
         A dh[VEC], dg[VEC];
@@ -613,27 +754,27 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
           for (int v = 0; v < VEC; ++v) dh[v] = 0;
         }
         round_pack(o, dh);
-        if (live) st_stream<T, VEC>(orow, o);
+        store_row(orow, o);
         if (want_gate) {
           A before[VEC];
-          widen<F, VEC>(before, FwdSlot::get(fs + r * kFwdRow, (fhalf + r * kodd) & 1));
+          if constexpr (RAGGED) widen<F, VEC>(before, Ragged<F, VEC>::get(fs + r * kFwdRow, col, moved(fat, r, dk, sizeof(F))));
+          else widen<F, VEC>(before, FwdSlot::get(fs + r * kFwdRow, moved(fat, r, dk, 1)));
           if (MARKED && (m & (kStart | kDead))) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) before[v] = 0;
-            if (live && (m & kStart)) load_acc<A, VEC>(before, p.init, (srow + (m >> kMarkBits)) * p.K + c0);
+            if (live && (m & kStart)) load_acc<A, VEC>(before, p.init, (srow + (m >> kMarkBits)) * p.K + c0, nv);
           }
           mul_all(dg, dh, before);
           if constexpr (!SHARED) {
             Pack<G, VEC> q;
             round_pack(q, dg);
-            if (live) st_stream<G, VEC>(grow, q);
+            store_row(grow, q);
           } else {
             // sum of the thread's channels, then of the neighbouring lanes that hold the same gate; the lanes of a row
             // are here together: rows are skipped (kPad) by whole rows
             A sum = dg[0];
 #pragma unroll
             for (int v = 1; v < VEC; ++v) sum += dg[v];
-            const unsigned rowmask = lx == 32 ? kFullMask : ((1u << lx) - 1u) << ((tid & 31) & ~(lx - 1));
             for (int d = 1; d < sum_lanes; d <<= 1) sum += __shfl_xor_sync(rowmask, sum, d);
             if (live && (col & (sum_lanes - 1)) == 0) {
               if (part_sums) *prow = sum;
@@ -646,7 +787,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
 #pragma unroll
           for (int v = 0; v < VEC; ++v) v_[v] = 0;
         }
-        if (MARKED && live && (m & kStart) && p.last) store_acc<A, VEC>(v_, p.last, (srow + (m >> kMarkBits)) * p.K + c0);
+        if (MARKED && live && (m & kStart) && p.last) store_acc<A, VEC>(v_, p.last, (srow + (m >> kMarkBits)) * p.K + c0, nv);
       }
     }
     };
@@ -661,15 +802,16 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
   for (int64_t done = 0; done < len; done += step) {
     load_rows(ahead_stage);
     async_wait_all_but<kStages - 1>();
+    if (RAGGED) __syncwarp();  // the chunks that the other lanes of a row copied are there
     tile_work(stage, par, set);
     tile += step;
     os += tile_k;
     ow += tile_k;
     og += tile_gates;
     op += step * dsums;
-    xhalf ^= xturn;
-    fhalf ^= xturn;
-    ghalf ^= gturn;
+    xat = moved(xat, step, dk, RAGGED ? sizeof(T) : 1);
+    fat = moved(fat, step, dk, RAGGED ? sizeof(F) : 1);
+    gat = moved(gat, step, dgates, RAGGED ? sizeof(G) : 1);
     stage = stage == kStages - 1 ? 0 : stage + 1;
     ahead_stage = ahead_stage == kStages - 1 ? 0 : ahead_stage + 1;
     set = set == kMarkStages - 1 ? 0 : set + 1;
@@ -717,9 +859,9 @@ inline int lanes_of_gate(int64_t width, int vec, int lx_log2) {
   return l;
 }
 
-template <typename T, typename G, int VEC, bool SHARED, bool BWD> int launch_tiles(ScanParams p, cudaStream_t stream) {
-  using S = ScanShape<T, G, VEC, SHARED, BWD>;
-  auto kernel = scan_kernel<T, G, VEC, SHARED, BWD>;
+template <typename T, typename G, int VEC, bool SHARED, bool BWD, bool RAGGED> int launch_tiles(ScanParams p, cudaStream_t stream) {
+  using S = ScanShape<T, G, VEC, SHARED, BWD, RAGGED>;
+  auto kernel = scan_kernel<T, G, VEC, SHARED, BWD, RAGGED>;
   static std::atomic<int> resident[64][8];  // CTAs of an SM by the lanes of a row; also: the attributes are set
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TSB_ERR_LAUNCH;
@@ -782,15 +924,6 @@ template <typename T, typename G, int VEC, bool SHARED, bool BWD> int launch_til
   return launch_status();
 }
 
-// The pack width: as many of a row's channels as 16 bytes hold, or 4 bytes, or one, by what the row length, the sharing
-// of the gate and the addresses allow.
-template <typename T> int pack_width(int64_t K, int64_t width, bool aligned16_all, bool aligned4_all) {
-  constexpr int full = full_vec<T>();
-  if (aligned16_all && K % full == 0 && (width == 1 || width % full == 0)) return full;
-  if (sizeof(T) == 2 && aligned4_all && K % 2 == 0 && (width == 1 || width % 2 == 0)) return 2;
-  return 1;
-}
-
 // Partial products of shared gates in a row, for whichever pack width the addresses will allow.
 inline int64_t partials_of_row(int64_t K, int64_t width, size_t elem) {
   int64_t most = 0;
@@ -818,16 +951,15 @@ template <typename T, typename G, bool BWD> int launch(const ScanParams &p, cuda
                                                                                              p.B, p.E, p.N, p.K, p.bstride);
   }
   if (p.E == 0) return launch_status();
-  const int vec = pack_width<T>(p.K, p.width, a16, a4);
-  const auto go = [&](auto v) {
-    constexpr int VEC = decltype(v)::value;
-    return p.width > 1 ? launch_tiles<T, G, VEC, true, BWD>(p, stream) : launch_tiles<T, G, VEC, false, BWD>(p, stream);
-  };
   constexpr int full = full_vec<T>();
-  if (vec == full) return go(std::integral_constant<int, full>());
+  // A gate of its own for every channel: 16 bytes of channels to a thread wherever the rows begin.  Shared gates: as many
+  // channels as 16 or 4 bytes hold if that divides the channels that share a gate, else one.
+  if (p.width == 1)
+    return a16 && p.K % full == 0 ? launch_tiles<T, G, full, false, BWD, false>(p, stream) : launch_tiles<T, G, full, false, BWD, true>(p, stream);
+  if (a16 && p.width % full == 0) return launch_tiles<T, G, full, true, BWD, false>(p, stream);
   if constexpr (sizeof(T) == 2)
-    if (vec == 2) return go(std::integral_constant<int, 2>());
-  return go(std::integral_constant<int, 1>());
+    if (a4 && p.width % 2 == 0) return launch_tiles<T, G, 2, true, BWD, false>(p, stream);
+  return launch_tiles<T, G, 1, true, BWD, false>(p, stream);
 }
 
 // one translation unit for each data type
