@@ -300,14 +300,13 @@ int tsb_expert_fold(const void *many, const int64_t *slot, const void *weight, c
  * scan_csr_backward: from grad_out [B,E,K] and grad_last [B,N,K] (either may be NULL: zero), and h (the forward's out, or
  *   wide with fp32 gates and 16-bit data; only read for grad_gate): grad_src [B,E,K] of dtype, grad_gate [B,E,K/width] of
  *   gate_dtype (or NULL), grad_state [B,N,K] (or NULL).
- *   workspace            tsb_scan_csr_backward_workspace_bytes(...) bytes, 256-byte aligned
+ *   workspace            tsb_scan_csr_backward_workspace_bytes(...) bytes, 256-byte aligned (0 unless width > 1)
  * Deterministic (no atomics).
  * scan_step: one token for each of n states: state[i,:] = gate[i,:] * state[i,:] + src[i,:] in place, out = the new
  * state rounded to dtype.  Consecutive states are state_stride elements apart (>= K). */
-size_t tsb_scan_csr_workspace_bytes(int64_t B, int64_t E, int64_t K, int64_t N, int64_t width, int dtype, int gate_dtype);
 int tsb_scan_csr(const void *src, const void *gate, const int64_t *indptr, const void *state, void *out, void *last,
                  void *wide, int64_t B, int64_t E, int64_t K, int64_t N, int64_t width, int64_t indptr_batch_stride, int dtype,
-                 int gate_dtype, void *workspace, size_t workspace_bytes, tsb_stream_t stream);
+                 int gate_dtype, tsb_stream_t stream);
 size_t tsb_scan_csr_backward_workspace_bytes(int64_t B, int64_t E, int64_t K, int64_t N, int64_t width, int dtype,
                                              int gate_dtype);
 int tsb_scan_csr_backward(const void *grad_out, const void *grad_last, const void *gate, const void *h,

@@ -50,11 +50,9 @@ int launch_tiles(const ScanParams &p, int dtype, int gate_dtype, bool backward, 
 
 using namespace tsb;
 
-extern "C" size_t tsb_scan_csr_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int, int) { return 0; }
-
 extern "C" int tsb_scan_csr(const void *src, const void *gate, const int64_t *indptr, const void *state, void *out, void *last,
                             void *wide, int64_t B, int64_t E, int64_t K, int64_t N, int64_t width, int64_t indptr_batch_stride, int dtype,
-                            int gate_dtype, void *, size_t, tsb_stream_t stream) {
+                            int gate_dtype, tsb_stream_t stream) {
   if (const int st = check(B, E, K, N, width, dtype, gate_dtype)) return st;
   if (B == 0 || K == 0 || (E == 0 && (N == 0 || !last))) return TSB_OK;
   if (!indptr || (E > 0 && (!src || !gate || !out))) return TSB_ERR_ARG;

@@ -9,7 +9,7 @@
 // Both are affine maps of the running value, value' = A * value + B, and maps compose: rows are cut into tiles of L rows,
 // and every input is read from HBM once.  A thread owns VEC channels (16 bytes) of R consecutive rows of a tile, which it
 // copies to its own slots of shared memory one tile ahead (cp.async; nobody else reads them, so the data needs no
-// barrier).  (1) It composes its rows' maps and leaves the result in shared memory.  (2) Turned over, a thread takes VEC
+// barrier; rows that begin off a 16-byte boundary are shared by a row's lanes, see Ragged).  (1) It composes its rows' maps and leaves the result in shared memory.  (2) Turned over, a thread takes VEC
 // consecutive maps of one channel, composes them and scans over the lanes that share the channel; the CTAs of a cluster
 // hold neighbouring tiles of the same channels and exchange their totals through distributed shared memory; then the
 // value that reaches each thread's rows is known.  (3) Each thread walks its rows again from that value and writes the

@@ -46,11 +46,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> scan_fw_impl(torch::Tens
   auto last = want_last ? state_like(src, indptr) : no_tensor(src);
   auto wide = want_wide ? torch::empty(src.sizes(), src.options().dtype(acc_dtype(src))) : no_tensor(src);
   BatchedRows rows = batched_rows(expand_indptr(indptr, src));
-  const size_t ws_bytes = tsb_scan_csr_workspace_bytes(d.B, d.E, d.K, d.N, d.width, dtype_enum(src), dtype_enum(gate));
-  auto workspace = torch::empty({(int64_t)ws_bytes}, src.options().dtype(torch::kUInt8));
   check_status(tsb_scan_csr(src.data_ptr(), gate.data_ptr(), rows.ptr(), opt_ptr(state), out.data_ptr(), want_last ? last.data_ptr() : nullptr,
-                            want_wide ? wide.data_ptr() : nullptr, d.B, d.E, d.K, d.N, d.width, rows.batch_stride, dtype_enum(src), dtype_enum(gate), workspace.data_ptr(), ws_bytes,
-                            current_stream()),
+                            want_wide ? wide.data_ptr() : nullptr, d.B, d.E, d.K, d.N, d.width, rows.batch_stride, dtype_enum(src), dtype_enum(gate), current_stream()),
                "tsb_scan_csr");
   return std::make_tuple(out, last, wide);
 }

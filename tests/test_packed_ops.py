@@ -130,10 +130,10 @@ def test_c_entries_report_errors_before_any_launch():
     assert lib.tsb_expert_fold(P, P, None, None, P, P, I(4), I(2), I(8), 0, None) == 3
     assert lib.tsb_expert_fold(None, None, None, None, None, None, I(0), I(2), I(8), 0, None) == 0
     shape = (I(1), I(6), I(8), I(3))
-    assert lib.tsb_scan_csr(P, P, P, None, P, None, None, *shape, I(3), I(0), 0, 0, P, size(1 << 20), None) == 3
-    assert lib.tsb_scan_csr(P, P, P, None, P, None, None, *shape, I(1), I(0), 0, 3, P, size(1 << 20), None) == 1
-    assert lib.tsb_scan_csr(P, P, None, None, P, None, None, *shape, I(1), I(0), 0, 0, P, size(1 << 20), None) == 3
-    assert lib.tsb_scan_csr(P, P, P, None, P, None, P, *shape, I(1), I(0), 0, 0, P, size(1 << 20), None) == 3
+    assert lib.tsb_scan_csr(P, P, P, None, P, None, None, *shape, I(3), I(0), 0, 0, None) == 3
+    assert lib.tsb_scan_csr(P, P, P, None, P, None, None, *shape, I(1), I(0), 0, 3, None) == 1
+    assert lib.tsb_scan_csr(P, P, None, None, P, None, None, *shape, I(1), I(0), 0, 0, None) == 3
+    assert lib.tsb_scan_csr(P, P, P, None, P, None, P, *shape, I(1), I(0), 0, 0, None) == 3
     assert lib.tsb_scan_csr_backward(P, None, P, None, P, None, P, P, None, *shape, I(1), I(0), 0, 0, P, size(1 << 20), None) == 3
     odd = (I(1), I(6), I(9), I(3))  # nine channels share a gate: their products are summed through the workspace
     assert lib.tsb_scan_csr_backward(P, None, P, P, P, None, P, P, None, *odd, I(9), I(0), 0, 0, None, size(0), None) == 4
