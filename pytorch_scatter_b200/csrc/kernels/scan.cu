@@ -6,16 +6,47 @@ namespace {
 
 using scan::ScanParams;
 
-template <typename T, typename G>
-__global__ void __launch_bounds__(kThreads) scan_step_kernel(const T *__restrict__ src, const G *__restrict__ gate, acc_t<T> *__restrict__ state,
-                                                             T *__restrict__ out, int64_t n, int64_t K, int64_t width, int64_t stride) {
-  for (int64_t it = (int64_t)blockIdx.x * kThreads + threadIdx.x; it < n * K; it += (int64_t)gridDim.x * kThreads) {
-    const int64_t i = it / K, c = it - i * K;
-    acc_t<T> &s = state[i * stride + c];
-    const acc_t<T> h = to_acc<G>(gate[i * (K / width) + c / width]) * s + to_acc<T>(src[it]);
-    s = h;
-    out[it] = from_acc<T>(h);
+// state = gate * state + src in place, one thread for VEC channels of a state.  Bound by HBM where there are enough states:
+// src, gate, state twice, out, each moved once.
+template <typename T, typename G, int VEC, bool SHARED>
+__global__ void __launch_bounds__(kThreads) scan_step_kernel(const T *src, const G *gate, acc_t<T> *state, T *out, int64_t n, int64_t K,
+                                                             int64_t width, int64_t stride) {
+  using A = acc_t<T>;
+  const int64_t Kv = K / VEC, items = n * Kv;
+  const bool small = items <= 0xffffffffLL;  // 32-bit divisions
+  for (int64_t it = (int64_t)blockIdx.x * kThreads + threadIdx.x; it < items; it += (int64_t)gridDim.x * kThreads) {
+    const int64_t i = small ? (int64_t)((unsigned)it / (unsigned)Kv) : it / Kv, c = (it - i * Kv) * VEC;
+    const Pack<T, VEC> x = ld_stream<T, VEC>(src + i * K + c);
+    Pack<A, VEC> s = ld_pack<A, VEC>(state + i * stride + c);
+    Pack<T, VEC> o;
+    if constexpr (SHARED) {
+      const A g = to_acc<G>(gate[i * (K / width) + (small ? (int64_t)((unsigned)c / (unsigned)width) : c / width)]);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) s.v[v] = g * s.v[v] + to_acc<T>(x.v[v]);
+    } else {
+      const Pack<G, VEC> g = ld_stream<G, VEC>(gate + i * K + c);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) s.v[v] = to_acc<G>(g.v[v]) * s.v[v] + to_acc<T>(x.v[v]);
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) o.v[v] = from_acc<T>(s.v[v]);
+    st_pack<A, VEC>(state + i * stride + c, s);
+    st_stream<T, VEC>(out + i * K + c, o);
   }
+}
+
+template <typename T, typename G>
+int launch_step(const T *src, const G *gate, acc_t<T> *state, T *out, int64_t n, int64_t K, int64_t width, int64_t stride, cudaStream_t stream) {
+  constexpr int VEC = 16 / (int)sizeof(acc_t<T>);  // 16 bytes of the state
+  const bool packs = K % VEC == 0 && (n <= 1 || stride % VEC == 0) && (width == 1 || width % VEC == 0) && aligned16(state) &&
+                     aligned16(src) && aligned16(out) && (width > 1 || aligned16(gate));
+  const auto go = [&](auto v, auto shared) {
+    constexpr int V = decltype(v)::value;
+    scan_step_kernel<T, G, V, decltype(shared)::value><<<scan::flat_blocks(n * (K / V)), kThreads, 0, stream>>>(src, gate, state, out, n, K, width, stride);
+    return launch_status();
+  };
+  const auto with_vec = [&](auto v) { return width > 1 ? go(v, std::true_type()) : go(v, std::false_type()); };
+  return packs ? with_vec(std::integral_constant<int, VEC>()) : with_vec(std::integral_constant<int, 1>());
 }
 
 template <typename F> int with_types(int dtype, int gate_dtype, F f) {
@@ -93,8 +124,7 @@ extern "C" int tsb_scan_step(const void *src, const void *gate, void *state, voi
   return with_types(dtype, gate_dtype, [&](auto t, auto g) -> int {
     using T = decltype(t);
     using G = decltype(g);
-    scan_step_kernel<T, G><<<scan::flat_blocks(n * K), kThreads, 0, (cudaStream_t)stream>>>(
-        static_cast<const T *>(src), static_cast<const G *>(gate), static_cast<acc_t<T> *>(state), static_cast<T *>(out), n, K, width, state_stride);
-    return launch_status();
+    return launch_step<T, G>(static_cast<const T *>(src), static_cast<const G *>(gate), static_cast<acc_t<T> *>(state), static_cast<T *>(out), n, K,
+                             width, state_stride, (cudaStream_t)stream);
   });
 }
