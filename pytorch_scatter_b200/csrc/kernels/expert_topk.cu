@@ -6,8 +6,8 @@
 // order of the logits is that of a 32-bit key, so that one warp reduction finds a maximum.  Bound by the instructions of
 // the choice, not by HBM: of a few hundred logits, most are ruled out first.  The k-th largest of the 32 lane maxima is a
 // lower bound of the k-th largest logit; the logits that reach it, rarely more than 2 k, move to one register of the
-// warp, and the k rounds of the choice run on that register.  (65536 x 256 fp32, k = 8: 53 us, 87 with every round
-// over all registers; the backward, which writes, 27.)
+// warp, and the k rounds of the choice run on that register.  (65536 x 256 fp32, k = 8: 50 us, 87 with every round
+// over all registers; the backward, which writes, 25.)
 #include "common.cuh"
 
 namespace tsb {
@@ -51,8 +51,11 @@ template <int R> __device__ __forceinline__ void softmax_stats(const Logits<R> &
   total = sum;
 }
 
-// Up to 32 rounds over all registers: lane j gets the j-th choice.  False: nothing was left for some of them.
-template <int R> __device__ __forceinline__ bool choose_all(unsigned (&key)[R], int n, int lane, unsigned &my_key, int &my_i) {
+// What a lane knows of a choice of up to 32: it holds the rank-th chosen expert (rank -1: none).
+struct Choice { unsigned key; int expert, rank; };
+
+// Up to 32 rounds over all registers; returns how many experts were chosen, fewer than n if nothing was left.
+template <int R> __device__ __forceinline__ int choose_all(unsigned (&key)[R], int n, int lane, Choice &mine) {
   for (int j = 0; j < n; ++j) {
     unsigned best = key[0];
     int at = lane;
@@ -60,28 +63,29 @@ template <int R> __device__ __forceinline__ bool choose_all(unsigned (&key)[R], 
     for (int r = 1; r < R; ++r)
       if (key[r] > best) { best = key[r]; at = r * 32 + lane; }
     const unsigned win = __reduce_max_sync(kFullMask, best);
-    if (win <= kNever) return false;
+    if (win <= kNever) return j;
     const int who = (int)__reduce_min_sync(kFullMask, best == win ? (unsigned)at : 0xffffffffu);
 #pragma unroll
     for (int r = 0; r < R; ++r)
       if (who == r * 32 + lane) key[r] = 0;
-    if (lane == j) { my_key = win; my_i = who; }
+    if (lane == j) mine = {win, who, j};
   }
-  return true;
+  return n;
 }
 
-// The same for n <= 32 through the candidates that reach the n-th largest lane maximum; false if they are more than 32
-// (equal logits), with nothing changed.
-template <int R> __device__ __forceinline__ bool choose_few(const unsigned (&key)[R], int n, int lane, uint2 *room, unsigned &my_key, int &my_i) {
+// The same for n <= 32 through the candidates that reach a lower bound of the n-th largest logit; -1 if they are more than
+// 32 (many equal logits), with nothing changed.  Candidates lie in the order of the experts, so of equal ones the first
+// lane's goes first.
+template <int R> __device__ __forceinline__ int choose_few(const unsigned (&key)[R], int n, int lane, uint2 *room, Choice &mine) {
   unsigned top = key[0];
 #pragma unroll
   for (int r = 1; r < R; ++r) top = max(top, key[r]);
-  unsigned bound = kNever + 1;
+  unsigned bound = kNever + 1;  // fewer than n lanes hold a logit that may be chosen: all of those are candidates
   for (int j = 0; j < n; ++j) {
     const unsigned win = __reduce_max_sync(kFullMask, top);
-    bound = max(win, kNever + 1);  // fewer than n lanes hold a logit that may be chosen: all of those are candidates
+    bound = max(win, kNever + 1);
     if (win <= kNever) break;
-    if (lane == __ffs(__ballot_sync(kFullMask, top == win)) - 1) top = 0;
+    if (top == win) top = 0;  // (equal maxima leave together: the bound is then lower than it could be)
   }
   int found = 0;
 #pragma unroll
@@ -93,16 +97,19 @@ template <int R> __device__ __forceinline__ bool choose_few(const unsigned (&key
     found += __popc(all);
   }
   __syncwarp();
-  if (found > 32) return false;
-  uint2 mine = lane < found ? room[lane] : make_uint2(0, 0xffffffffu);
+  if (found > 32) return -1;
+  const uint2 own = lane < found ? room[lane] : make_uint2(0, 0);
+  mine = {own.x, (int)own.y, -1};
+  unsigned left = own.x;
   for (int j = 0; j < n; ++j) {
-    const unsigned win = __reduce_max_sync(kFullMask, mine.x);
-    if (win <= kNever) break;
-    const unsigned who = __reduce_min_sync(kFullMask, mine.x == win ? mine.y : 0xffffffffu);
-    if (mine.y == who) mine.x = 0;
-    if (lane == j) { my_key = win; my_i = (int)who; }
+    const unsigned win = __reduce_max_sync(kFullMask, left);
+    if (win <= kNever) return j;
+    if (lane == __ffs(__ballot_sync(kFullMask, left == win)) - 1) {
+      left = 0;
+      mine.rank = j;
+    }
   }
-  return true;
+  return n;
 }
 
 template <typename T, int R>
@@ -125,24 +132,33 @@ __global__ void __launch_bounds__(kThreads) topk_kernel(const T *__restrict__ lo
     float chosen = 0.0f;
     for (int j0 = 0; j0 < k; j0 += 32) {
       const int n = min(32, k - j0);
-      unsigned my_key = 0;
-      int my_i = -1;
-      bool done = false;
+      Choice mine{0, -1, -1};
+      int found = -1;
       if constexpr (R > 2)
-        if (k <= 32) done = choose_few<R>(key, n, lane, room, my_key, my_i);
-      if (!done) choose_all<R>(key, n, lane, my_key, my_i);
-      const float v = key_value(my_key);
-      if (normalize && j0 == 0) top = __shfl_sync(kFullMask, v, 0);  // the largest of all
-      const float p = my_i < 0 ? 0.0f : expf(v - top);
+        if (k <= 32) found = choose_few<R>(key, n, lane, room, mine);
+      if (found < 0) {
+        mine = {0, -1, -1};
+        found = choose_all<R>(key, n, lane, mine);
+      }
+      const float v = key_value(mine.key);
+      if (normalize && j0 == 0) {  // the largest of all
+        const unsigned first = __ballot_sync(kFullMask, mine.rank == 0);
+        top = __shfl_sync(kFullMask, v, first ? __ffs(first) - 1 : 0);
+      }
+      const float p = mine.rank < 0 ? 0.0f : expf(v - top);
       if (normalize) {
         float sum = p;
 #pragma unroll
         for (int s = 16; s; s >>= 1) sum += shfl_xor(sum, s);
         chosen += sum;
       }
-      if (lane < n) {
-        index[t * k + j0 + lane] = my_i;
-        weight[t * k + j0 + lane] = my_i < 0 ? 0.0f : k <= 32 ? p / (normalize ? chosen : den) : p;
+      if (mine.rank >= 0) {
+        index[t * k + j0 + mine.rank] = mine.expert;
+        weight[t * k + j0 + mine.rank] = k <= 32 ? p / (normalize ? chosen : den) : p;
+      }
+      if (lane >= found && lane < n) {
+        index[t * k + j0 + lane] = -1;
+        weight[t * k + j0 + lane] = 0.0f;
       }
     }
     if (k > 32) {
