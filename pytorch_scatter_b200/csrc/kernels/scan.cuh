@@ -447,11 +447,12 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
         }
         __syncwarp();
         // borders from the first row's segment on, 32 at a time, until one is beyond the tile
-        for (int64_t s0 = BWD ? u : u - 1;; s0 += BWD ? -32 : 32) {
+        for (int64_t s0 = BWD ? u : u - 1;;) {
           const int64_t s = BWD ? s0 - lane : s0 + lane;
           bool beyond = s < 0 || s > p.N;
+          int64_t at = -1;
           if (!beyond) {
-            const int64_t at = indptr[s];
+            at = indptr[s];
             beyond = BWD ? at < low : at > high + 1;
             if (at >= low && at <= high && s < p.N && indptr[s + 1] > at)
               atomicOr(&mark[BWD ? high - at : at - low], (int)s << kMarkBits | kStart);
@@ -459,6 +460,13 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
               atomicOr(&mark[BWD ? high - (at - 1) : at - 1 - low], (int)(s - 1) << kMarkBits | kEnd);
           }
           if (__any_sync(kFullMask, beyond && (BWD ? s <= p.N : s >= 0))) break;
+          // a run of empty segments at one row: on to its last border, the only other one that matters
+          const long long at0 = __shfl_sync(kFullMask, (long long)at, 0), at31 = __shfl_sync(kFullMask, (long long)at, 31);
+          s0 += BWD ? -32 : 32;
+          if (at0 == at31) {
+            const int64_t end = BWD ? bound<false>(indptr, 0, s0 + 1, at0) : bound<true>(indptr, s0, p.N + 1, at0) - 1;
+            s0 = BWD ? (end < s0 ? end : s0) : (end > s0 ? end : s0);
+          }
         }
       }
       if (lane == 0) s_marked[stage] = !plain;

@@ -429,6 +429,21 @@ def test_scan_many_empty_segments_and_a_long_stream():
     assert torch.equal(out.cpu(), row.float().unsqueeze(1).expand(E, 8))
 
 
+def test_scan_runs_of_empty_segments():
+    """Hundreds of thousands of empty segments at one row, at the first row and behind the last, forward and backward."""
+    ends = torch.cat([torch.zeros(100001, dtype=torch.long), torch.tensor([37]), torch.full((300000,), 50), torch.tensor([51, 90, 90]),
+                      torch.full((1000,), 130)])
+    N, src, gate = ends.numel() - 1, torch.ones(140, 4, device='cuda').requires_grad_(), torch.ones(140, 4, device='cuda')
+    out, last = ts.scan_csr_state(src, gate, ends.cuda())
+    lens = ends[1:] - ends[:-1]
+    row = torch.arange(130) - torch.repeat_interleave(ends[:-1], lens) + 1
+    assert torch.equal(out[:130].cpu(), row.float().unsqueeze(1).expand(130, 4)) and not bool(out[130:].any())
+    assert torch.equal(last[:, 0].cpu(), lens.float()) and last.shape == (N, 4)
+    (g,) = torch.autograd.grad(out, src, torch.ones_like(out))
+    behind = torch.repeat_interleave(ends[1:], lens) - torch.arange(130)  # rows from here to the segment's end
+    assert torch.equal(g[:130].cpu(), behind.float().unsqueeze(1).expand(130, 4)) and not bool(g[130:].any())
+
+
 def test_scan_empty_shapes():
     z = torch.zeros
     p = torch.tensor([0, 0, 0], device='cuda')
