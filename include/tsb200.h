@@ -296,9 +296,9 @@ int tsb_expert_fold(const void *many, const int64_t *slot, const void *weight, c
  *   gate_dtype           dtype, or TSB_F32 with 16-bit data
  *   out                  rows outside every segment become 0
  *   last                 h at each segment's last row; state[n] (or 0) for empty segments
- *   wide                 h in fp32 as well, [B,E,K], for the backward with fp32 gates and 16-bit data; NULL otherwise
- * scan_csr_backward: from grad_out [B,E,K] and grad_last [B,N,K] (either may be NULL: zero), and h (the forward's out, or
- *   wide with fp32 gates and 16-bit data; only read for grad_gate): grad_src [B,E,K] of dtype, grad_gate [B,E,K/width] of
+ *   wide                 16-bit data: h in fp32 as well, [B,E,K], for grad_gate; NULL if not wanted, and with other data
+ * scan_csr_backward: from grad_out [B,E,K] and grad_last [B,N,K] (either may be NULL: zero), and h (the forward's wide
+ *   with 16-bit data, else its out; only read for grad_gate): grad_src [B,E,K] of dtype, grad_gate [B,E,K/width] of
  *   gate_dtype (or NULL), grad_state [B,N,K] (or NULL).
  *   workspace            tsb_scan_csr_backward_workspace_bytes(...) bytes, 256-byte aligned (0 unless width > 1)
  * Deterministic (no atomics).

@@ -88,7 +88,7 @@ extern "C" int tsb_scan_csr(const void *src, const void *gate, const int64_t *in
   if (B == 0 || K == 0 || (E == 0 && (N == 0 || !last))) return TSB_OK;
   if (!indptr || (E > 0 && (!src || !gate || !out))) return TSB_ERR_ARG;
   ScanParams p{};
-  if (wide && gate_dtype == dtype) return TSB_ERR_ARG;
+  if (wide && dtype != TSB_F16 && dtype != TSB_BF16) return TSB_ERR_ARG;
   p.src = src; p.gate = gate; p.state = state; p.indptr = indptr; p.out = out; p.last = last; p.wide = wide;
   p.B = B; p.E = E; p.K = K; p.N = N; p.width = width; p.bstride = indptr_batch_stride;
   return launch_tiles(p, dtype, gate_dtype, false, stream);

@@ -17,8 +17,8 @@
 // on by its CTAs' tiles, carrying the value along in registers, so that one launch covers any length without waiting on
 // anything but its own cluster.  The composition has a fixed shape: results do not vary from run to run.
 //
-// 65536 x 2048 bf16 in 37 segments: forward 174 us, 4.6 TB/s, backward 269 us, 5.0 TB/s; bound by the latency of a tile's
-// chain of steps with eight warps on an SM, and by HBM where no border breaks it (one segment of 65536 x 4096: 5.5 TB/s).
+// 65536 x 2048 bf16 in 37 segments: forward 176 us, 4.6 TB/s, with h kept in 32 bits for a backward 298 us, 4.5 TB/s,
+// backward 318 us, 5.1 TB/s; bound by the latency of a tile's chain of steps with eight warps on an SM.
 //
 // A segment's first row (backward: its last) does not take the value from the row before: such a map is marked `reset`
 // and drops what comes in, so infinities and NaN of one segment never reach the next.  Tiles that no segment border
@@ -40,7 +40,7 @@ constexpr int kMostCluster = 8;
 
 struct ScanParams {
   const void *src, *gate, *state;  // backward: src = grad_out (may be null), state = grad_last
-  const void *fwd, *init;          // backward: the forward's h and state
+  const void *fwd, *init;          // backward: the forward's h in the accumulation type, and its state
   const int64_t *indptr;
   void *out, *last;                // backward: grad_src, grad_state
   void *grad_gate, *partial;       // backward
@@ -84,8 +84,8 @@ template <typename T, int VEC> struct Slot {
   }
 };
 
-// Rows that begin anywhere (60000 x 333 fp16 in 3001 segments, forward / backward: 126 / 187 us; one channel to a thread
-// instead: 191 / 369): the lanes of a row share its aligned 16-byte chunks, n of them to a lane and one more, and a
+// Rows that begin anywhere (60000 x 333 fp16 in 3001 segments, forward / backward: 126 / 204 us; one channel to a thread
+// instead: 191 / 369, the latter with h in 16 bits): the lanes of a row share its aligned 16-byte chunks, n of them to a lane and one more, and a
 // lane shifts its values out of its own and the next one (the lanes of a row are lanes of one warp).
 template <typename X, int VEC> struct Ragged {
   static constexpr int n = (int)sizeof(X) * VEC / 16;
@@ -350,13 +350,12 @@ __device__ __forceinline__ void send(unsigned addr, unsigned bar, double a, doub
 template <typename T, typename G, int VEC, bool SHARED, bool BWD, bool RAGGED> struct ScanShape {
   using A = acc_t<T>;
   static constexpr int kGateVec = SHARED ? 1 : VEC;
-  // The backward multiplies dh by the h before it.  With a gate of the data's type that is the rounded output: the
-  // gradient, which is rounded to the same type, then carries two such roundings.  A wider gate has a gradient in 32 bits,
-  // which the rounding of h would spoil: its backward reads h as the recurrence held it.
-  using F = std::conditional_t<(sizeof(G) > sizeof(T)), A, T>;
+  // The backward multiplies dh by the h before it as the recurrence held it, not by the rounded output, whose rounding
+  // the gradient would carry besides its own (relative error against 64 bits 2.3e-3 instead of 1.7e-3 in bf16, 2.9e-4
+  // instead of 2.1e-4 in fp16).  With 16-bit data the forward writes h a second time for it, in 32 bits.
   using SrcSlot = Slot<T, VEC>;
   using GateSlot = Slot<G, kGateVec>;
-  using FwdSlot = Slot<F, VEC>;
+  using FwdSlot = Slot<A, VEC>;
   static constexpr int kRowBytes = SrcSlot::kBytes + (BWD ? FwdSlot::kBytes : 0) + GateSlot::kBytes;
   // Rows of a thread: 42 KB for each of the two stages at most, so that two CTAs fit an SM.  What a tile costs besides its
   // rows, step (2), is then a small part (65536 x 4096 bf16: 291 us with 10 rows and 2 stages, 302 with 7 rows and 3
@@ -381,7 +380,6 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
   using SrcSlot = typename S::SrcSlot;
   using GateSlot = typename S::GateSlot;
   using FwdSlot = typename S::FwdSlot;
-  using F = typename S::F;
   using A = acc_t<T>;
   constexpr int R = S::kRows;
   // A ragged row is a few hundred instructions: unrolled, the loops over a thread's rows do not fit the instruction cache
@@ -494,7 +492,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
   const int64_t srow = b * p.N;                     // first row of this batch in the state arrays
   const bool have_src = !BWD || p.src, want_gate = BWD && p.grad_gate;
   const T *src_lo = static_cast<const T *>(p.src), *src_hi = src_lo + p.B * p.E * p.K;
-  const F *fwd_lo = static_cast<const F *>(p.fwd), *fwd_hi = fwd_lo + p.B * p.E * p.K;
+  const A *fwd_lo = static_cast<const A *>(p.fwd), *fwd_hi = fwd_lo + p.B * p.E * p.K;
   const G *gate_lo = static_cast<const G *>(p.gate), *gate_hi = gate_lo + p.B * p.E * gates;
 
   // this thread's slots [stage][row][thread], and its pointers to the next tile to load and to the tile at work
@@ -505,7 +503,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
   int64_t ahead = tile + ty * R;                    // position of the thread's next rows to load
   const int64_t at = b * p.E + row_of(ahead);
   const T *lsrc = src_lo + (have_src ? at * p.K + c0 : 0);
-  const F *lfwd = fwd_lo + (BWD ? (at - 1) * p.K + c0 : 0);  // h of the row before
+  const A *lfwd = fwd_lo + (BWD ? (at - 1) * p.K + c0 : 0);  // h of the row before
   const G *lgate = gate_lo + at * gates + g0;
   T *os = static_cast<T *>(p.out) + at * p.K + c0;
   A *ow = static_cast<A *>(p.wide) + (!BWD && p.wide ? at * p.K + c0 : 0);
@@ -531,7 +529,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
     if (RAGGED) __syncwarp();  // the lanes of a row have read each other's chunks of this stage
     if ((live || (RAGGED && (col - 1) * VEC < tile_c)) && left > 0) {  // (a ragged row may end in the chunk of the lane behind)
       const T *xs = lsrc;
-      const F *fs = lfwd;
+      const A *fs = lfwd;
       const G *gs = lgate;
       char *xd = s_src + stage * (R * kSrcRow), *fd = s_fwd + stage * (R * kFwdRow), *gd = s_gate + stage * (R * kGateRow);
       const int n = left < R ? (int)left : R;
@@ -544,7 +542,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
           if constexpr (RAGGED) {
             if (have_src) Ragged<T, VEC>::copy(xd + r * kSrcRow, xs - kcol, col, lx, tile_c * (int)sizeof(T), edge, src_lo, src_hi);
             Ragged<G, VEC>::copy(gd + r * kGateRow, gs - kcol, col, lx, tile_c * (int)sizeof(G), edge, gate_lo, gate_hi);
-            if (BWD && want_gate && fs - kcol >= fwd_lo) Ragged<F, VEC>::copy(fd + r * kFwdRow, fs - kcol, col, lx, tile_c * (int)sizeof(F), edge, fwd_lo, fwd_hi);
+            if (BWD && want_gate && fs - kcol >= fwd_lo) Ragged<A, VEC>::copy(fd + r * kFwdRow, fs - kcol, col, lx, tile_c * (int)sizeof(A), edge, fwd_lo, fwd_hi);
           } else {
           if (have_src) SrcSlot::copy(xd + r * kSrcRow, xs, edge, src_lo, src_hi);
           GateSlot::copy(gd + r * kGateRow, gs, edge, gate_lo, gate_hi);
@@ -747,14 +745,17 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
         }
         round_pack(o, v_);
         store_row(orow, o);
-        if (live) {
-          if constexpr (!std::is_same<F, T>::value)
-            if (p.wide) {
-              if (RAGGED) store_acc<A, VEC>(v_, wrow, 0, nv);
-              else store_wide(wrow, v_);
+        if constexpr (!std::is_same<A, T>::value)
+          if (p.wide) {
+            if constexpr (RAGGED) {
+              Pack<A, VEC> w;
+              round_pack(w, v_);
+              store_row(wrow, w);
+            } else if (live) {
+              store_wide(wrow, v_);
             }
-          if (MARKED && (m & kEnd) && p.last) store_acc<A, VEC>(v_, p.last, (srow + (m >> kMarkBits)) * p.K + c0, nv);
-        }
+          }
+        if (MARKED && live && (m & kEnd) && p.last) store_acc<A, VEC>(v_, p.last, (srow + (m >> kMarkBits)) * p.K + c0, nv);
       } else {
         A dh[VEC], dg[VEC];
 #pragma unroll
@@ -768,8 +769,8 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
         store_row(orow, o);
         if (want_gate) {
           A before[VEC];
-          if constexpr (RAGGED) widen<F, VEC>(before, Ragged<F, VEC>::get(fs + r * kFwdRow, col, moved(fat, r, dk, sizeof(F))));
-          else widen<F, VEC>(before, FwdSlot::get(fs + r * kFwdRow, moved(fat, r, dk, 1)));
+          if constexpr (RAGGED) widen<A, VEC>(before, Ragged<A, VEC>::get(fs + r * kFwdRow, col, moved(fat, r, dk, sizeof(A))));
+          else widen<A, VEC>(before, FwdSlot::get(fs + r * kFwdRow, moved(fat, r, dk, 1)));
           if (MARKED && (m & (kStart | kDead))) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) before[v] = 0;
@@ -821,7 +822,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
     og += tile_gates;
     op += step * dsums;
     xat = moved(xat, step, dk, RAGGED ? sizeof(T) : 1);
-    fat = moved(fat, step, dk, RAGGED ? sizeof(F) : 1);
+    fat = moved(fat, step, dk, RAGGED ? sizeof(A) : 1);
     gat = moved(gat, step, dgates, RAGGED ? sizeof(G) : 1);
     stage = stage == kStages - 1 ? 0 : stage + 1;
     ahead_stage = ahead_stage == kStages - 1 ? 0 : ahead_stage + 1;

@@ -66,10 +66,12 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> scan_bw_impl(std::option
   auto grad_gate = want_gate ? torch::empty_like(gate) : no_tensor(gate);
   auto grad_state = want_state ? state_like(out, indptr) : no_tensor(out);
   BatchedRows rows = batched_rows(expand_indptr(indptr, out));
+  TORCH_CHECK(!want_gate || wide.has_value() || out.scalar_type() == acc_dtype(out), "scan_csr: the gradient of the gate needs h in the accumulation type");
+  const void *h = !want_gate ? nullptr : wide.has_value() ? wide.value().data_ptr() : out.data_ptr();
   const size_t ws_bytes = tsb_scan_csr_backward_workspace_bytes(d.B, d.E, d.K, d.N, d.width, dtype_enum(out), dtype_enum(gate));
   auto workspace = torch::empty({(int64_t)ws_bytes}, out.options().dtype(torch::kUInt8));
   check_status(tsb_scan_csr_backward(opt_ptr(grad_out), opt_ptr(grad_last), gate.data_ptr(),
-                                     wide.has_value() ? wide.value().data_ptr() : out.data_ptr(), rows.ptr(), opt_ptr(state),
+                                     h, rows.ptr(), opt_ptr(state),
                                      grad_src.data_ptr(), want_gate ? grad_gate.data_ptr() : nullptr, want_state ? grad_state.data_ptr() : nullptr,
                                      d.B, d.E, d.K, d.N, d.width, rows.batch_stride, dtype_enum(out), dtype_enum(gate), workspace.data_ptr(), ws_bytes,
                                      current_stream()),
@@ -155,8 +157,8 @@ variable_list scan(const char *name, torch::Tensor src, torch::Tensor gate, torc
     auto r = scan_fw(src, gate, indptr, state, want_last, false);
     return {std::get<0>(r), std::get<1>(r)};
   }
-  // with a gate wider than the data the gradient of the gate needs h unrounded (see the kernel)
-  const bool want_wide = gate.scalar_type() != src.scalar_type() && gate.requires_grad();
+  // the gradient of the gate needs h as the recurrence held it (see the kernel)
+  const bool want_wide = src.scalar_type() != acc_dtype(src) && gate.requires_grad();
   return ScanCSR::apply(src, gate, indptr, state, want_last, want_wide);
 }
 

@@ -22,8 +22,8 @@ def scan_csr(src: torch.Tensor, gate: torch.Tensor, indptr: torch.Tensor,
             float64 data).
 
     The recurrence runs in 32 bits (64 for float64) whatever the data's type and is rounded once per output.  Rows
-    outside every range are 0 and get no gradient.  With float32 gates and 16-bit data a forward pass that will need
-    the gates' gradient keeps ``h`` in float32 as well.  Differentiable (once) with respect to ``src``, ``gate`` and
+    outside every range are 0 and get no gradient.  With 16-bit data a forward pass that will need the gates' gradient
+    keeps ``h`` in float32 as well.  Differentiable (once) with respect to ``src``, ``gate`` and
     ``state``; bit-reproducible run to run.
     """
     return torch.ops.torch_scatter.scan_csr(src, gate, indptr, state)
