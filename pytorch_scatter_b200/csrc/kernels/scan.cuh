@@ -969,8 +969,8 @@ template <typename T, typename G, bool BWD> int launch(const ScanParams &p, cuda
   if (p.width == 1)
     return a16 && p.K % full == 0 ? launch_tiles<T, G, full, false, BWD, false>(p, stream) : launch_tiles<T, G, full, false, BWD, true>(p, stream);
   if (a16 && p.width % full == 0) return launch_tiles<T, G, full, true, BWD, false>(p, stream);
-  if constexpr (sizeof(T) == 2)
-    if (a4 && p.width % 2 == 0) return launch_tiles<T, G, 2, true, BWD, false>(p, stream);
+  if constexpr (sizeof(T) == 2)  // (two channels of the h that the backward reads are 8 bytes)
+    if (a4 && (reinterpret_cast<uintptr_t>(p.fwd) & 7) == 0 && p.width % 2 == 0) return launch_tiles<T, G, 2, true, BWD, false>(p, stream);
   return launch_tiles<T, G, 1, true, BWD, false>(p, stream);
 }
 

@@ -1,8 +1,11 @@
 """Edges of the packed-batch operators on the GPU: how exact the gate's gradient is, data at any address, infinities,
 offsets beyond the rows, places without an entry.  Tolerances count roundings (see packed_ref.py)."""
+import ctypes
+
 import pytest
 import torch
 
+import cabi
 import packed_ref as ref
 import pytorch_scatter_b200 as ts
 
@@ -44,3 +47,48 @@ def test_gate_gradient_of_16_bit_data_is_rounded_once(heads, width, dtype):
     got = torch.autograd.grad(out, xg, grad.cuda())[0]
     assert got.dtype == dtype and out.dtype == dtype
     ref.assert_within(got, want, err + ref.last_rounding(want, dtype), 'grad_gate')
+
+
+def at_offset(t, nbytes):
+    """The tensor's values `nbytes` behind a 256-byte boundary, with as much room behind them."""
+    n = t.numel() * t.element_size()
+    buf = torch.zeros(n + nbytes + 256, dtype=torch.uint8, device='cuda')
+    room = buf[nbytes:nbytes + n].view(t.dtype)
+    assert buf.data_ptr() % 256 == 0 and room.data_ptr() % 256 == nbytes
+    return room.view(t.shape).copy_(t)
+
+
+@pytest.mark.parametrize('dtype,gdtype', [(BF16, F32), (BF16, BF16), (F16, F32), (F32, F32)])
+@pytest.mark.parametrize('heads,width', [(3, 6), (2, 8), (1, 33), (24, 1)])
+@pytest.mark.parametrize('data_off,h_off', [(0, 4), (0, 8), (4, 4), (4, 8), (8, 12), (4, 16)])
+def test_raw_pointers_at_any_address_of_their_type(data_off, h_off, heads, width, dtype, gdtype):
+    """The C entries, with every array where its type alone allows it and h (fp32) on another boundary than the data: two
+    16-bit channels are 4 bytes, two of h are 8."""
+    gen = torch.Generator().manual_seed(heads + width)
+    E, K, ends = 170, heads * width, [0, 60, 170]
+    src, grad = rand(gen, E, heads, width, dtype=dtype), rand(gen, E, heads, width, dtype=dtype)
+    gate = torch.sigmoid(rand(gen, E, heads, 1) + 2).to(gdtype)
+    x, d, g = at_offset(src, data_off), at_offset(grad, data_off), at_offset(gate, 4)
+    out, dx, dg = at_offset(torch.zeros_like(src), data_off), at_offset(torch.zeros_like(src), data_off), at_offset(torch.zeros_like(gate), 4)
+    wide = at_offset(torch.zeros(E, K), h_off) if dtype != F32 else None
+    p, lib, dt = torch.tensor(ends, device='cuda'), cabi.lib(), (cabi.DTYPE[dtype], cabi.DTYPE[gdtype])
+    shape = [cabi._i(v) for v in (1, E, K, 2, width, 0)]
+    ptr = cabi._p
+    cabi._check(lib.tsb_scan_csr(ptr(x), ptr(g), ptr(p), None, ptr(out), None, ptr(wide), *shape, *dt, cabi._stream()), 'tsb_scan_csr')
+    h = wide if wide is not None else at_offset(out.cpu(), h_off)
+    need = lib.tsb_scan_csr_backward_workspace_bytes
+    need.restype = ctypes.c_size_t
+    n = need(*shape[:5], *dt)
+    ws = torch.empty(n + 1, dtype=torch.uint8, device='cuda')
+    cabi._check(lib.tsb_scan_csr_backward(ptr(d), None, ptr(g), ptr(h), ptr(p), None, ptr(dx), ptr(dg), None, *shape, *dt, ptr(ws),
+                                          ctypes.c_size_t(n), cabi._stream()), 'tsb_scan_csr_backward')
+    torch.cuda.synchronize()
+    flat = lambda t: t.double().expand(E, heads, width).reshape(E, K)  # noqa: E731
+    want, before, _, mass, way = ref.scan(flat(src), flat(gate), ends, None)
+    dh, _, _, dmass, dway, _, _ = ref.scan_backward(flat(grad), None, flat(gate), before, ends)
+    u = ref.unit(F32)
+    ref.assert_within(out.reshape(E, K), want, u * (4 * way + 32 * mass) + ref.last_rounding(want, dtype), 'out')
+    ref.assert_within(h.reshape(E, K), want, u * (4 * way + 32 * mass), 'h')
+    ref.assert_within(dx.reshape(E, K), dh, u * (4 * dway + 32 * dmass) + ref.last_rounding(dh, dtype), 'grad_src')
+    total, err = gate_gradient(src, gate, grad, ends)
+    ref.assert_within(dg, total, err + ref.last_rounding(total, gdtype), 'grad_gate')
