@@ -114,7 +114,10 @@ public:
     TORCH_CHECK(false, "torch_scatter: this operator has no second derivative");
   }
 };
+// Whether the tensor carries a forward-mode derivative, which these operators do not have.
+inline bool has_tangent(const torch::Tensor &t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
 inline torch::autograd::variable_list first_order(torch::autograd::variable_list grads, std::vector<torch::Tensor> from) {
+  for (auto &t : from) TORCH_CHECK(!has_tangent(t), "torch_scatter: the gradient of this operator has no forward-mode derivative");
   if (!at::GradMode::is_enabled()) return grads;
   std::vector<torch::Tensor> known;
   for (auto &t : from)
@@ -134,7 +137,10 @@ inline void check_float_dtype(const torch::Tensor &t, const char *name) {
               name, " must be a float32, float64, float16 or bfloat16 tensor, got ", s);
 }
 // No gradient can be asked for: the operator is called without an autograd node around it (2 us of the host's time).
+// Forward-mode derivatives go through the node, which refuses them, also under no_grad.
 inline bool no_grad_for(std::initializer_list<torch::Tensor> ts) {
+  for (auto &t : ts)
+    if (has_tangent(t)) return false;
   if (!at::GradMode::is_enabled()) return true;
   for (auto &t : ts)
     if (t.defined() && t.requires_grad()) return false;

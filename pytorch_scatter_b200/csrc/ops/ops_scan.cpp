@@ -193,6 +193,7 @@ torch::Tensor scan_step(torch::Tensor src, torch::Tensor gate, torch::Tensor sta
   gate = checked_gate("scan_step", src, gate, 0);
   TORCH_CHECK(!at::GradMode::is_enabled() || !(src.requires_grad() || gate.requires_grad() || state.requires_grad()),
               "scan_step updates the state in place and has no gradient: call it under torch.no_grad(), or scan_csr_state for training");
+  TORCH_CHECK(!has_tangent(src) && !has_tangent(gate) && !has_tangent(state), "scan_step has no forward-mode derivative");
   if (src.numel() > 0) {
     int64_t K = 1;  // inside a state the elements are dense; consecutive states may lie apart
     for (int64_t i = src.dim() - 1; i >= 1; i--) {

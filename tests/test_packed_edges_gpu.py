@@ -92,3 +92,18 @@ def test_raw_pointers_at_any_address_of_their_type(data_off, h_off, heads, width
     ref.assert_within(dx.reshape(E, K), dh, u * (4 * dway + 32 * dmass) + ref.last_rounding(dh, dtype), 'grad_src')
     total, err = gate_gradient(src, gate, grad, ends)
     ref.assert_within(dg, total, err + ref.last_rounding(total, gdtype), 'grad_gate')
+
+
+def test_tangents_of_incoming_gradients_raise():
+    """Forward over reverse: a backward pass whose incoming gradient carries a tangent."""
+    fwd = torch.autograd.forward_ad
+    slot, _, p = ts.expert_sort(torch.tensor([[0, 1], [1, 2], [2, 0], [0, 2]], device='cuda'), 3)
+    x = torch.randn(4, 6, device='cuda', requires_grad=True)
+    for f in (lambda: ts.expert_topk(x, 2)[0], lambda: ts.expert_dispatch(x, slot, p), lambda: ts.expert_combine(torch.cat([x, x]), slot, p),
+              lambda: ts.scan_csr(x, torch.sigmoid(x), torch.tensor([0, 1, 4], device='cuda'))):
+        with fwd.dual_level():
+            y = f()
+            for again in (False, True):
+                g = fwd.make_dual(torch.ones_like(y), torch.ones_like(y))
+                with pytest.raises(RuntimeError, match='forward-mode|jvp'):
+                    torch.autograd.grad(y, x, g, retain_graph=True, create_graph=again)
