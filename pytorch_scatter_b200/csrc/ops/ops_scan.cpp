@@ -20,6 +20,7 @@ ScanDims scan_dims(const torch::Tensor &src, const torch::Tensor &gate, const to
     d.K *= src.size(i);
     if (gate.size(i) != src.size(i)) d.width *= src.size(i);
   }
+  if (d.K == 0) d.width = 1;  // gates that no channel shares
   return d;
 }
 
@@ -64,6 +65,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> scan_bw_impl(std::option
   const ScanDims d = scan_dims(out, gate, indptr);
   auto grad_src = torch::empty_like(out);
   auto grad_gate = want_gate ? torch::empty_like(gate) : no_tensor(gate);
+  if (want_gate && d.K == 0) grad_gate.zero_();  // empty sums: a shared gate exists without channels
   auto grad_state = want_state ? state_like(out, indptr) : no_tensor(out);
   BatchedRows rows = batched_rows(expand_indptr(indptr, out));
   TORCH_CHECK(!want_gate || wide.has_value() || out.scalar_type() == acc_dtype(out), "scan_csr: the gradient of the gate needs h in the accumulation type");

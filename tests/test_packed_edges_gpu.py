@@ -107,3 +107,23 @@ def test_tangents_of_incoming_gradients_raise():
                 g = fwd.make_dual(torch.ones_like(y), torch.ones_like(y))
                 with pytest.raises(RuntimeError, match='forward-mode|jvp'):
                     torch.autograd.grad(y, x, g, retain_graph=True, create_graph=again)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('shape,gate_shape', [((4, 3, 0), (4, 3, 1)), ((4, 0, 5), (4, 1, 1)), ((4, 0, 5), (4, 0, 1)), ((4, 3, 0), (4, 1, 1)),
+                                              ((0, 3, 0), (0, 3, 1)), ((4, 3, 0), (4, 3, 0)), ((4, 0), (4, 1))])
+def test_scan_of_no_channels(shape, gate_shape, dtype):
+    """Shared gates of rows without channels: empty outputs, and gradients of zero where the gates exist."""
+    p = torch.tensor([0, shape[0] // 2, shape[0]], device='cuda')
+    src = torch.zeros(shape, dtype=dtype, device='cuda', requires_grad=True)
+    gate = torch.ones(gate_shape, dtype=dtype, device='cuda', requires_grad=True)
+    state = torch.zeros((2,) + shape[1:], device='cuda', requires_grad=True)
+    out, last = ts.scan_csr_state(src, gate, p, state)
+    assert out.shape == shape and out.dtype == dtype and last.shape == state.shape
+    assert ts.scan_csr(src.detach(), gate.detach(), p).shape == shape
+    torch.full((64,), float('nan'), device='cuda')  # (what a gradient left unwritten might hold)
+    gs, gg, gst = torch.autograd.grad((out, last), (src, gate, state), (torch.ones_like(out), torch.ones_like(last)))
+    assert gs.shape == shape and gst.shape == state.shape and torch.equal(gg, torch.zeros_like(gate))
+    if shape[0]:
+        with torch.no_grad():
+            assert ts.scan_step(src[:2], gate[:2], state.detach()).shape == (2,) + shape[1:]
