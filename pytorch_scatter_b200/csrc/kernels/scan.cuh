@@ -295,10 +295,21 @@ template <typename T, int VEC, typename A> __device__ __forceinline__ void round
   }
 }
 
-// A product of gates may overflow where the recurrence itself stays at zero: kept finite, so that A * 0 + B = B.
-template <typename A> __device__ __forceinline__ A finite(A a) {
-  constexpr A most = std::numeric_limits<A>::max();
-  return a > most ? most : a < -most ? -most : a;
+// A product of gates, brought back into the range of numbers.  It may overflow where the recurrence itself stays at zero:
+// kept finite, so that A * 0 + B = B.  One that underflows keeps the smallest magnitude unless a gate is 0 (`zero`): an
+// infinite value that comes in stays infinite, as it does row by row, and only a gate of 0 makes it NaN.  (A finite value
+// times the smallest magnitude is off by less than one step of the product of the two.)  NaN stays NaN.
+__device__ __forceinline__ float in_range(float a, bool zero) {
+  const float least = zero ? 0.0f : __int_as_float(1);
+  float r;
+  asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(std::numeric_limits<float>::max()));
+  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(r), "f"(least));
+  return r;
+}
+__device__ __forceinline__ double in_range(double a, bool zero) {
+  constexpr double most = std::numeric_limits<double>::max();
+  a = a > most ? most : a < -most ? -most : a;
+  return a == 0 && !zero ? copysign(std::numeric_limits<double>::denorm_min(), a) : a;
 }
 
 // A map that drops what comes in travels between CTAs with this A, which no product of gates can be.
@@ -636,19 +647,35 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
         if constexpr (SHARED) ma[0] *= g[0];
         else mul_all(ma, ma, g);
       }
-      A *pa = s_a + own_map, *pb = s_b + own_map;
+      bool gates = true;  // no product is 0
+#pragma unroll
+      for (int v = 0; v < (SHARED ? 1 : VEC); ++v) {
+        ma[v] = in_range(ma[v], true);
+        gates = gates && (ma[v] != 0 || (RAGGED && v >= nv));
+      }
       if constexpr (SHARED) {
 #pragma unroll
         for (int v = 1; v < VEC; ++v) ma[v] = ma[0];
       }
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) ma[v] = finite(ma[v]);
-      put(pa, ma);
-      put(pb, mb);
+      put(s_a + own_map, ma);
+      put(s_b + own_map, mb);
       if (marked && col == 0) s_reset[ty] = reset;
+      return gates || !live;
     };
-    if (mine) map_rows(std::true_type());
-    else map_rows(std::false_type());
+    if (!(mine ? map_rows(std::true_type()) : map_rows(std::false_type()))) {
+      // was a gate of the thread's rows 0, or are they small?
+      unsigned zeros = 0;
+#pragma unroll 1
+      for (int r = 0; r < R; ++r) {
+        if (mine && (mark[r] & (kPad | kDead))) continue;
+        A x[VEC], g[VEC];
+        read_row(x, g, r);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) zeros |= (unsigned)(g[v] == 0) << v;
+      }
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) s_a[own_map + v] = in_range(s_a[own_map + v], zeros >> v & 1);
+    }
     __syncthreads();
 
     // ---- (2) scan of the maps over the tile and the cluster
@@ -662,20 +689,22 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
     }
     A ta = fa[0], tb = fb[0];
     int tr = fr & 1;
+    bool zero = ta == 0;
 #pragma unroll
     for (int j = 1; j < VEC; ++j) {
       const bool rs = marked && (fr >> j & 1);
       tb = rs ? fb[j] : fa[j] * tb + fb[j];
       ta *= fa[j];
+      zero = zero || fa[j] == 0;
       tr |= rs;
     }
-    ta = finite(ta);
+    ta = in_range(ta, zero);
     for (int d = 1; d < H; d <<= 1) {
       const A pa = __shfl_up_sync(kFullMask, ta, d, H), pb = __shfl_up_sync(kFullMask, tb, d, H);
       const int pr = marked ? __shfl_up_sync(kFullMask, tr, d, H) : 0;
       if (fh >= d) {
         if (!tr) tb = ta * pb + tb;
-        ta = finite(ta * pa);
+        ta = in_range(ta * pa, ta == 0 || pa == 0);
         tr |= pr;
       }
     }

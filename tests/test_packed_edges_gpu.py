@@ -127,3 +127,50 @@ def test_scan_of_no_channels(shape, gate_shape, dtype):
     if shape[0]:
         with torch.no_grad():
             assert ts.scan_step(src[:2], gate[:2], state.detach()).shape == (2,) + shape[1:]
+
+
+def same_kind(got, want, what):
+    """NaN, +inf and -inf at the same places."""
+    got = got.detach().cpu().double()
+    assert torch.equal(got.isnan(), want.isnan()), f'{what}: NaN'
+    assert torch.equal(got == float('inf'), want == float('inf')) and torch.equal(got == -float('inf'), want == -float('inf')), f'{what}: infinities'
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F64])
+@pytest.mark.parametrize('heads,width', [(40, 1), (7, 1), (3, 16), (1, 33)])
+@pytest.mark.parametrize('decay', [0.5, -0.5, 1e-3, 1e-12, 0.0])
+def test_infinite_values_stay_infinite(decay, heads, width, dtype):
+    """An infinity stays one under gates that are not 0, however small their product; a gate of 0 makes it NaN.  Over
+    sequences that a thread, a tile and a cluster of tiles hold."""
+    gen = torch.Generator().manual_seed(heads)
+    ends, H, P = [0, 12, 400, 6400], heads, width
+    E, inf = ends[-1], float('inf')
+    src, grad = rand(gen, E, H, P, dtype=dtype), rand(gen, E, H, P, dtype=dtype)
+    gate = torch.full((E, H, 1), 0.75).to(dtype)
+    gate[::3] = decay if decay else 0.75
+    if not decay:
+        gate[[8, 300, 3000]] = 0.0
+    for lo, hi in zip(ends[:-1], ends[1:]):
+        src[lo + (hi - lo) // 4, 0, 0], src[lo + (hi - lo) // 2, H - 1, P - 1] = inf, -inf
+        grad[hi - 1 - (hi - lo) // 4, 0, 0], grad[hi - 1 - (hi - lo) // 2, H - 1, P - 1] = -inf, inf
+    flat = lambda t: t.double().expand(E, H, P).reshape(E, H * P)  # noqa: E731
+    want, before, last, mass, way = ref.scan(flat(src), flat(gate), ends, None)
+    dh, dg, _, dmass, dway, _, _ = ref.scan_backward(flat(grad), None, flat(gate), before, ends)
+    assert bool(want.isinf().any()) and bool(dh.isinf().any()) and bool(want.isnan().any()) == (decay == 0)
+    xs, xg = src.cuda().requires_grad_(), gate.cuda().requires_grad_()
+    out, state = ts.scan_csr_state(xs, xg, torch.tensor(ends, device='cuda'))
+    gs, gg = torch.autograd.grad(out, (xs, xg), grad.cuda())
+    same_kind(out.reshape(E, H * P), want, 'out')
+    same_kind(state.reshape(3, H * P), last, 'last')
+    same_kind(gs.reshape(E, H * P), dh, 'grad_src')
+    # An infinite dh times an h whose roundings reach 0 may be infinite or NaN, and so may an infinite h times such a dh:
+    # with bf16 data 0.75 a + b is exactly 0 for some a and b, and the 1e-12 of the row before them, which 64 bits still hold
+    # next to a, is below half a step of 32 bits.  Both are within u (4 way + 32 mass) of their values, so only where that
+    # reaches 0 is nothing asked.
+    u = ref.unit(dtype)
+    may_be_0 = lambda v, by: v.isfinite() & (v != 0) & (v.abs() <= by)  # noqa: E731
+    unsure = dh.isinf() & may_be_0(before, torch.roll(u * (4 * way + 32 * mass), 1, 0))
+    unsure |= before.isinf() & may_be_0(dh, u * (4 * dway + 32 * dmass))
+    assert int(unsure.sum()) < unsure.numel() // 100
+    sure = ~unsure.reshape(E, H, P).any(-1, keepdim=True)
+    same_kind(gg.cpu()[sure], dg.reshape(E, H, P).sum(-1, keepdim=True)[sure], 'grad_gate')
