@@ -439,7 +439,8 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
   // ---- the fifth warp: where segments begin and end, one tile ahead of the others
   if (tid >= kScanThreads) {
     const int lane = tid - kScanThreads;
-    const int64_t first = indptr[0], behind = indptr[p.N];
+    const auto border = [&](int64_t s) { return clamp64(indptr[s], 0, p.E); };  // (offsets beyond the rows end at them)
+    const int64_t first = border(0), behind = border(p.N);
     int64_t cursor = BWD ? p.N + 1 : 0;  // bound of the row looked up last
     const auto look = [&](int64_t tile, int stage) {
       // the segment of the tile's first row on the way: does it hold the whole tile, without beginning or ending in it?
@@ -447,7 +448,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
       const int64_t u = BWD ? bound<true>(indptr, 0, cursor, from) : bound<true>(indptr, cursor, p.N + 1, from);
       cursor = u;
       const int64_t low = BWD ? to : from, high = BWD ? from : to;
-      const bool plain = tile + L <= len && u >= 1 && u <= p.N && indptr[u - 1] < low && indptr[u] > high + 1;
+      const bool plain = tile + L <= len && u >= 1 && u <= p.N && border(u - 1) < low && border(u) > high + 1;
       if (!plain) {
         int *mark = s_marks + stage * L;
         for (int j = lane; j < L; j += 32) {
@@ -461,11 +462,11 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
           bool beyond = s < 0 || s > p.N;
           int64_t at = -1;
           if (!beyond) {
-            at = indptr[s];
+            at = border(s);
             beyond = BWD ? at < low : at > high + 1;
-            if (at >= low && at <= high && s < p.N && indptr[s + 1] > at)
+            if (at >= low && at <= high && s < p.N && border(s + 1) > at)
               atomicOr(&mark[BWD ? high - at : at - low], (int)s << kMarkBits | kStart);
-            if (at > low && at <= high + 1 && s > 0 && indptr[s - 1] < at)
+            if (at > low && at <= high + 1 && s > 0 && border(s - 1) < at)
               atomicOr(&mark[BWD ? high - (at - 1) : at - 1 - low], (int)(s - 1) << kMarkBits | kEnd);
           }
           if (__any_sync(kFullMask, beyond && (BWD ? s <= p.N : s >= 0))) break;

@@ -174,3 +174,25 @@ def test_infinite_values_stay_infinite(decay, heads, width, dtype):
     assert int(unsure.sum()) < unsure.numel() // 100
     sure = ~unsure.reshape(E, H, P).any(-1, keepdim=True)
     same_kind(gg.cpu()[sure], dg.reshape(E, H, P).sum(-1, keepdim=True)[sure], 'grad_gate')
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('K', [64, 7])
+@pytest.mark.parametrize('ends', [[-3, 20, 90, 130], [-9, -4, 100, 300], [0, 40, 128, 129, 140], [-50, 200], [130, 140], [-7, -2, 0, 100]])
+def test_scan_offsets_beyond_the_rows(ends, K, dtype):
+    """A segment that reaches over the rows' ends is what of it lies inside, as in segment_csr: its state comes in at its
+    first row, its last state and the gradient of its state are written."""
+    gen = torch.Generator().manual_seed(K)
+    E, N = 100, len(ends) - 1
+    inside = [min(max(e, 0), E) for e in ends]
+    src, grad = rand(gen, E, K, dtype=dtype).cuda(), rand(gen, E, K, dtype=dtype).cuda()
+    gate = torch.sigmoid(rand(gen, E, K)).to(dtype).cuda()
+    state, grad_last = rand(gen, N, K).cuda(), rand(gen, N, K).cuda()
+
+    def both(offsets):
+        leaves = [t.clone().requires_grad_() for t in (src, gate, state)]
+        out, last = ts.scan_csr_state(leaves[0], leaves[1], torch.tensor(offsets, device='cuda'), leaves[2])
+        return (out.detach(), last.detach()) + torch.autograd.grad((out, last), leaves, (grad, grad_last))
+
+    for got, want, what in zip(both(ends), both(inside), ('out', 'last', 'grad_src', 'grad_gate', 'grad_state')):
+        assert torch.equal(got, want), what
