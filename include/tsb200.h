@@ -277,7 +277,8 @@ int tsb_expert_sort(const int64_t *index, int64_t *slot, int64_t *order, int64_t
                     void *workspace, size_t workspace_bytes, tsb_stream_t stream);
 
 /* expert_spread: many[slot[t,j], :] = few[t, :] (* weight[t,j]).  few [T,K], slot [T,k], many [T*k, K]; fp32 / fp64 /
- * fp16 / bf16.  Rows of many from *used (device pointer: indptr[E]) on are zeroed; slots outside [0, T*k) are skipped.
+ * fp16 / bf16.  Rows of many from *used (device pointer: indptr[E]) on, and rows before it that no slot names, are zeroed;
+ * slots outside [0, T*k) are skipped, no two of the others may be equal.
  *   weight               [T,k] in the accumulation type (fp32, fp64 for fp64 data) or NULL
  *   rows, dot            both or neither: dot[t,j] = <few[t,:], rows[slot[t,j],:]> (accumulation type, 0 where the slot
  *                        is skipped), the gradient of the weights; rows [T*k, K] of dtype

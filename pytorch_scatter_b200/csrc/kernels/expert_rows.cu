@@ -9,8 +9,15 @@
 // Rows move in 16-byte chunks.  Where the row length is no multiple of 16 bytes, chunks are those of the row that is
 // written, and the data comes out of the two aligned chunks of the source row that hold it, shifted into place: twice the
 // load instructions, but whole sectors and 16-byte stores instead of single values.
+//
+// Rows of many that no slot names are zeroed: those behind the last expert's, and those inside whose entries were dropped
+// after the sort (a capacity limit).  Up to kOneList entries a few blocks of the spread look all slots up for the rows that
+// they guard; beyond that a second kernel first counts the slots, since usually there are as many as rows (3 to 5 us).
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <atomic>
+#include <utility>
 
 #include "mbarrier.cuh"
 
@@ -25,6 +32,7 @@ struct RowsParams {
   const void *weight;
   void *few_out, *many_out, *dot;
   int64_t T, k, K, M;
+  int zero_blocks;           // spread with ZERO: the first blocks zero the rows that no slot names
 };
 
 template <typename T> constexpr int chunk_len() { return 16 / (int)sizeof(T); }
@@ -157,8 +165,92 @@ template <typename T, bool ALIGNED> __device__ __forceinline__ void zero_tail(co
   for (int64_t i = first; i < (p.M - used) * p.K / V; i += step) st_stream<T, V>(tail + i * V, zero);
 }
 
+// zeros for the rows [lo, hi) of many that no slot names, by a whole CTA
+constexpr int64_t kOneList = 4096;  // entries
+template <typename T, bool ALIGNED, int WORDS>
+__device__ __forceinline__ void zero_unnamed(const RowsParams &p, int64_t lo, int64_t hi, unsigned (&s_named)[WORDS]) {
+  constexpr int V = ALIGNED ? chunk_len<T>() : 1;
+  Pack<T, V> zero;
+#pragma unroll
+  for (int i = 0; i < V; ++i) zero.v[i] = from_acc<T>((acc_t<T>)0);
+  for (; lo < hi; lo += WORDS * 32) {
+    const int n = (int)(hi - lo < WORDS * 32 ? hi - lo : WORDS * 32);
+    for (int i = threadIdx.x; i * 32 < n; i += blockDim.x) s_named[i] = 0;
+    __syncthreads();
+#pragma unroll 8
+    for (int64_t i = threadIdx.x; i < p.M; i += blockDim.x) {
+      const uint64_t r = (uint64_t)(p.slot[i] - lo);  // (slots below lo are beyond n, too)
+      if (r < (uint64_t)n) atomicOr(&s_named[r >> 5], 1u << (r & 31));
+    }
+    __syncthreads();
+    for (int r = threadIdx.x >> 5; r < n; r += blockDim.x >> 5) {
+      if (s_named[r >> 5] >> (r & 31) & 1) continue;
+      T *row = static_cast<T *>(p.many_out) + (lo + r) * p.K;
+      for (int64_t c = threadIdx.x & 31; c < p.K / V; c += 32) st_stream<T, V>(row + c * V, zero);
+    }
+    __syncthreads();
+  }
+}
+// The block's part where the first blocks do that; true: the block has nothing else to do.
+template <typename T, bool ALIGNED> __device__ __forceinline__ bool zero_part(const RowsParams &p) {
+  if ((int)blockIdx.x >= p.zero_blocks) return false;
+  __shared__ unsigned s_named[kOneList / 32];
+  const int64_t per = (p.M + p.zero_blocks - 1) / p.zero_blocks, lo = blockIdx.x * per;
+  zero_unnamed<T, ALIGNED>(p, lo, lo + per < p.M ? lo + per : p.M, s_named);
+  return true;
+}
+
+// Many entries: next to the spread, which zeroes the rows from *used on.  Every cluster counts the slots; are there fewer than
+// rows, its CTAs look them up for parts of the rows.  Launched to start while the spread's last CTAs run (the two write
+// different rows, and what this one reads was there before the spread began), and over when the spread is.
+constexpr int kHoleThreads = 1024, kHoleCluster = 8, kHoleWords = 2048;
+template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kHoleThreads) __cluster_dims__(kHoleCluster) holes_kernel(RowsParams p) {
+  namespace cg = cooperative_groups;
+  __shared__ unsigned s_named[kHoleWords];
+  __shared__ unsigned s_warp[kHoleThreads / 32];
+  __shared__ int64_t s_counts[kHoleCluster];
+  auto cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank();
+  auto all_run = cluster.barrier_arrive();
+  const int64_t used = clamp64(*p.used, 0, p.M);
+  unsigned named = 0;
+#pragma unroll 8
+  for (int64_t i = rank * kHoleThreads + (int)threadIdx.x; i < p.M; i += kHoleCluster * kHoleThreads) named += (uint64_t)p.slot[i] < (uint64_t)used;
+  named = __reduce_add_sync(kFullMask, named);
+  if ((threadIdx.x & 31) == 0) s_warp[threadIdx.x >> 5] = named;
+  __syncthreads();
+  cluster.barrier_wait(std::move(all_run));
+  if (threadIdx.x < kHoleCluster) {
+    int64_t sum = 0;
+    for (int w = 0; w < kHoleThreads / 32; ++w) sum += s_warp[w];
+    *cluster.map_shared_rank(&s_counts[rank], threadIdx.x) = sum;
+  }
+  cluster.sync();  // (nobody leaves before all others have written to its shared memory)
+  int64_t count = 0;
+#pragma unroll
+  for (int q = 0; q < kHoleCluster; ++q) count += s_counts[q];
+  if (count != used) {
+    const int64_t per = (used + gridDim.x - 1) / gridDim.x, lo = blockIdx.x * per;
+    zero_unnamed<T, ALIGNED>(p, lo, lo + per < used ? lo + per : used, s_named);
+  }
+  cudaGridDependencySynchronize();  // the spread is over and its rows are there before this kernel is over
+}
+template <typename T, bool ALIGNED> int launch_holes(const RowsParams &p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(kHoleCluster * std::max<int64_t>(1, std::min<int64_t>(16, p.M / 16384))));
+  cfg.blockDim = dim3(kHoleThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, holes_kernel<T, ALIGNED>, p) == cudaSuccess ? TSB_OK : TSB_ERR_LAUNCH;
+}
+
 // Without dot products: one thread, one chunk of one token.  The rows of several choices are in flight at once.
-template <typename T, bool SPREAD, bool ALIGNED>
+// ZERO (in code of its own: with it the kernel takes 64 registers instead of 46): see zero_part.
+template <typename T, bool SPREAD, bool ALIGNED, bool ZERO>
 __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
   using A = acc_t<T>;
   constexpr int V = chunk_len<T>(), J = 4;
@@ -166,7 +258,11 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
   const T *few_in = static_cast<const T *>(p.few_in), *many_in = static_cast<const T *>(p.many_in);
   T *few_out = static_cast<T *>(p.few_out), *many_out = static_cast<T *>(p.many_out);
   const int64_t Kc = chunks_of<T, ALIGNED>(p.K), items = p.T * Kc;
-  const int64_t step = (int64_t)gridDim.x * kThreads, first = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if constexpr (SPREAD && !ZERO) cudaTriggerProgrammaticLaunchCompletion();  // holes_kernel may start
+  if constexpr (ZERO)
+    if (zero_part<T, ALIGNED>(p)) return;
+  const int skip = ZERO ? p.zero_blocks : 0;
+  const int64_t step = (int64_t)(gridDim.x - skip) * kThreads, first = (int64_t)(blockIdx.x - skip) * kThreads + threadIdx.x;
   for (int64_t it = first; it < items; it += step) {
     const int64_t t = items <= 0xffffffffLL ? (int64_t)((unsigned)it / (unsigned)Kc) : it / Kc, c = it - t * Kc;
     const int64_t *slot = p.slot + t * p.k;
@@ -223,13 +319,13 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(RowsParams p) {
       store_span<T>(row + e0, o, s);
     }
   }
-  if constexpr (SPREAD) zero_tail<T, ALIGNED>(p, first, step);
+  if constexpr (SPREAD && !ZERO) zero_tail<T, ALIGNED>(p, first, step);
 }
 
 // With dot products: G threads (lanes of a warp, or the CTA) walk one token's chunks, J choices at a time.  WRITE: also
 // spread or fold; a fold needs all choices of a chunk at once, so it has J >= k.  Unaligned chunks take
 // twice the registers, so fewer choices are in flight.
-template <typename T, bool SPREAD, bool ALIGNED, bool WRITE, int J, int G>
+template <typename T, bool SPREAD, bool ALIGNED, bool WRITE, bool ZERO, int J, int G>
 __global__ void __launch_bounds__(kThreads) rows_dot_kernel(RowsParams p) {
   using A = acc_t<T>;
   constexpr int V = chunk_len<T>(), kGroups = kThreads / G, kWarps = kThreads / 32;
@@ -240,8 +336,12 @@ __global__ void __launch_bounds__(kThreads) rows_dot_kernel(RowsParams p) {
   A *dot = static_cast<A *>(p.dot);
   const int64_t Kc = chunks_of<T, ALIGNED>(p.K);
   const int lane = threadIdx.x % G, group = threadIdx.x / G;
+  if constexpr (SPREAD && !ZERO) cudaTriggerProgrammaticLaunchCompletion();
+  if constexpr (ZERO)
+    if (zero_part<T, ALIGNED>(p)) return;
+  const int skip = ZERO ? p.zero_blocks : 0;
   // whole warps stay together: the last round of tokens may hold groups without one
-  for (int64_t t0 = (int64_t)blockIdx.x * kGroups; t0 < p.T; t0 += (int64_t)gridDim.x * kGroups) {
+  for (int64_t t0 = (int64_t)(blockIdx.x - skip) * kGroups; t0 < p.T; t0 += (int64_t)(gridDim.x - skip) * kGroups) {
     const int64_t t = t0 + group;
     const bool live = t < p.T;
     for (int64_t j0 = 0; j0 < p.k; j0 += J) {
@@ -325,7 +425,7 @@ __global__ void __launch_bounds__(kThreads) rows_dot_kernel(RowsParams p) {
       }
     }
   }
-  if constexpr (SPREAD && WRITE) zero_tail<T, ALIGNED>(p, (int64_t)blockIdx.x * kThreads + threadIdx.x, (int64_t)gridDim.x * kThreads);
+  if constexpr (SPREAD && !ZERO) zero_tail<T, ALIGNED>(p, (int64_t)blockIdx.x * kThreads + threadIdx.x, (int64_t)gridDim.x * kThreads);
 }
 
 // Folds, and spreads with dot products, of long aligned rows of many tokens.  Every warp runs a pipeline of its own: bulk
@@ -345,6 +445,7 @@ __global__ void __launch_bounds__(kBulkWarps * 32, 2) rows_bulk_kernel(RowsParam
   constexpr int V = chunk_len<T>(), U = kBulkChunks;
   extern __shared__ __align__(128) char s_ring[];
   __shared__ __align__(8) uint64_t s_bar[kBulkWarps][kBulkMostStages];
+  if constexpr (SPREAD) cudaTriggerProgrammaticLaunchCompletion();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = (int)p.k;
   const unsigned ring = smem_at(s_ring) + warp * kBulkWarpBytes, bar = smem_at(&s_bar[warp][0]);
   const char *ring_p = s_ring + warp * kBulkWarpBytes;
@@ -492,12 +593,12 @@ template <typename T, bool SPREAD, bool DOT> int launch_bulk(const RowsParams &p
   return launch_status();
 }
 
-template <typename T, bool SPREAD, bool ALIGNED, bool WRITE> int launch_dot(const RowsParams &p, cudaStream_t stream) {
+template <typename T, bool SPREAD, bool ALIGNED, bool WRITE, bool ZERO> int launch_dot(const RowsParams &p, cudaStream_t stream) {
   const auto go = [&](auto jn, auto gn) {
     constexpr int J = decltype(jn)::value, G = decltype(gn)::value;
     const int64_t want = (p.T + kThreads / G - 1) / (kThreads / G);
     const int64_t blocks = std::min<int64_t>(want, (int64_t)sm_count() * 32);
-    rows_dot_kernel<T, SPREAD, ALIGNED, WRITE, J, G><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
+    rows_dot_kernel<T, SPREAD, ALIGNED, WRITE, ZERO, J, G><<<(unsigned)blocks + p.zero_blocks, kThreads, 0, stream>>>(p);
     return launch_status();
   };
   const auto with_j = [&](auto gn) {
@@ -513,20 +614,35 @@ template <typename T, bool SPREAD, bool ALIGNED, bool WRITE> int launch_dot(cons
   return with_j(std::integral_constant<int, kThreads>());
 }
 
-template <typename T, bool SPREAD, bool ALIGNED> int launch_rows(const RowsParams &p, cudaStream_t stream) {
-  if constexpr (ALIGNED) {
-    BulkShape shape;
-    if (p.dot && bulk_shape<T, true>(p, shape)) return launch_bulk<T, SPREAD, true>(p, shape, stream);
-    if constexpr (!SPREAD)
-      if (!p.dot && bulk_shape<T, false>(p, shape)) return launch_bulk<T, false, false>(p, shape, stream);
-  }
-  if (p.dot && (SPREAD || p.k <= (ALIGNED ? 8 : 4))) return launch_dot<T, SPREAD, ALIGNED, true>(p, stream);
+template <typename T, bool SPREAD, bool ALIGNED, bool ZERO> int launch_moves(const RowsParams &p, cudaStream_t stream) {
+  if (p.dot && (SPREAD || p.k <= (ALIGNED ? 8 : 4))) return launch_dot<T, SPREAD, ALIGNED, true, ZERO>(p, stream);
   const int64_t items = p.T * chunks_of<T, ALIGNED>(p.K);
   const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((int64_t)sm_count() * 64, (items + kThreads - 1) / kThreads));
-  rows_kernel<T, SPREAD, ALIGNED><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
+  rows_kernel<T, SPREAD, ALIGNED, ZERO><<<(unsigned)blocks + p.zero_blocks, kThreads, 0, stream>>>(p);
   if constexpr (!SPREAD)
-    if (p.dot) return launch_dot<T, SPREAD, ALIGNED, false>(p, stream);
+    if (p.dot) return launch_dot<T, SPREAD, ALIGNED, false, false>(p, stream);
   return launch_status();
+}
+
+template <typename T, bool SPREAD, bool ALIGNED> int launch_rows(RowsParams p, cudaStream_t stream) {
+  BulkShape shape;
+  if constexpr (!SPREAD) {
+    if constexpr (ALIGNED) {
+      if (p.dot && bulk_shape<T, true>(p, shape)) return launch_bulk<T, false, true>(p, shape, stream);
+      if (!p.dot && bulk_shape<T, false>(p, shape)) return launch_bulk<T, false, false>(p, shape, stream);
+    }
+    return launch_moves<T, false, ALIGNED, false>(p, stream);
+  } else {
+    const bool bulk = ALIGNED && p.dot && bulk_shape<T, true>(p, shape);
+    if (!bulk && p.M <= kOneList) {
+      p.zero_blocks = (int)std::min<int64_t>(128, (p.M + 63) / 64);
+      return launch_moves<T, true, ALIGNED, true>(p, stream);
+    }
+    int st;
+    if constexpr (ALIGNED) st = bulk ? launch_bulk<T, true, true>(p, shape, stream) : launch_moves<T, true, true, false>(p, stream);
+    else st = launch_moves<T, true, false, false>(p, stream);
+    return st == TSB_OK ? launch_holes<T, ALIGNED>(p, stream) : st;
+  }
 }
 
 template <bool SPREAD> int rows_entry(const RowsParams &p, int dtype, cudaStream_t stream) {
@@ -559,7 +675,7 @@ extern "C" int tsb_expert_spread(const void *few, const int64_t *slot, const int
   if (T < 0 || k < 1 || K < 0 || (K > 0 && (rows != nullptr) != (dot != nullptr))) return TSB_ERR_ARG;
   if (T == 0) return TSB_OK;
   if (!slot || (K > 0 && (!few || !many || !used))) return TSB_ERR_ARG;
-  return rows_entry<true>({few, rows, slot, used, weight, nullptr, many, dot, T, k, K, T * k}, dtype, (cudaStream_t)stream);
+  return rows_entry<true>({few, rows, slot, used, weight, nullptr, many, dot, T, k, K, T * k, 0}, dtype, (cudaStream_t)stream);
 }
 
 extern "C" int tsb_expert_fold(const void *many, const int64_t *slot, const void *weight, const void *other, void *few,
@@ -567,6 +683,6 @@ extern "C" int tsb_expert_fold(const void *many, const int64_t *slot, const void
   if (T < 0 || k < 1 || K < 0 || (K > 0 && (other != nullptr) != (dot != nullptr))) return TSB_ERR_ARG;
   if (T == 0) return TSB_OK;
   if (!slot || (K > 0 && (!few || !many))) return TSB_ERR_ARG;
-  return rows_entry<false>({other, many, slot, nullptr, weight, few, nullptr, dot, T, k, K, T * k}, dtype,
+  return rows_entry<false>({other, many, slot, nullptr, weight, few, nullptr, dot, T, k, K, T * k, 0}, dtype,
                            (cudaStream_t)stream);
 }

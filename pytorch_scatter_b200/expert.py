@@ -52,10 +52,11 @@ def expert_dispatch(src: torch.Tensor, slot: torch.Tensor, indptr: torch.Tensor,
 
     Args:
         src: ``[*tokens, ...]`` float32, float64, float16 or bfloat16 (CUDA).
-        slot, indptr: as :func:`expert_sort` returned them, ``slot`` ``[*tokens, k]``.
+        slot, indptr: as :func:`expert_sort` returned them, ``slot`` ``[*tokens, k]``.  Entries may be dropped afterwards
+            by a slot of -1; two entries must not share a slot.
         weight: optional factors of ``slot``'s shape, float32 (float64 with float64 rows).
 
-    Returns ``[slot.numel(), ...]``; rows behind ``indptr[-1]`` are zero.  Differentiable (once) with respect to ``src``
+    Returns ``[slot.numel(), ...]``; rows that no entry names, those behind ``indptr[-1]`` among them, are zero.  Differentiable (once) with respect to ``src``
     and ``weight``; bit-reproducible run to run.
     """
     return torch.ops.torch_scatter.expert_dispatch(src, slot, indptr, weight)
@@ -68,7 +69,8 @@ def expert_combine(rows: torch.Tensor, slot: torch.Tensor, indptr: torch.Tensor,
     Args:
         rows: ``[slot.numel(), ...]`` float32, float64, float16 or bfloat16 (CUDA); rows behind ``indptr[-1]`` are not
             read.
-        slot, indptr: as :func:`expert_sort` returned them, ``slot`` ``[*tokens, k]``.
+        slot, indptr: as :func:`expert_sort` returned them, ``slot`` ``[*tokens, k]``.  Entries may be dropped afterwards
+            by a slot of -1 (their rows get a gradient of zero); two entries must not share a slot.
         weight: optional factors of ``slot``'s shape, float32 (float64 with float64 rows).
 
     Returns ``[*tokens, ...]``; tokens whose entries were all dropped are zero.  Differentiable (once) with respect to

@@ -196,3 +196,102 @@ def test_scan_offsets_beyond_the_rows(ends, K, dtype):
 
     for got, want, what in zip(both(ends), both(inside), ('out', 'last', 'grad_src', 'grad_gate', 'grad_state')):
         assert torch.equal(got, want), what
+
+
+def leave_nan(*sizes):
+    """Memory of these sizes (bytes) that the next allocations will probably get, full of NaN."""
+    blocks = [torch.full((n // 4 + 1,), float('nan'), device='cuda') for n in sizes]
+    torch.cuda.synchronize()
+    del blocks
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F64])
+@pytest.mark.parametrize('T,k,K', [(1, 1, 5), (6, 2, 64), (40, 3, 129), (700, 8, 256), (1000, 8, 33), (1025, 8, 40), (30000, 4, 16), (9000, 2, 7),
+                                   (2400, 2, 1032), (2400, 8, 520)])
+@pytest.mark.parametrize('drop', ['some', 'one expert', 'all'])
+def test_rows_that_no_entry_names_are_zero(T, k, K, drop, dtype):
+    """Entries dropped after the sort, as a capacity limit does it: holes among the rows, in few and many entries, in every
+    way that the rows move (with and without weights, with their gradient, rows off a 16-byte boundary)."""
+    gen = torch.Generator().manual_seed(T + k + K)
+    index = torch.randint(-1, 7, (T, k), generator=gen)
+    slot, _, indptr = ts.expert_sort(index.cuda(), 7)
+    gone = {'some': torch.rand(T, k, generator=gen) < 0.3, 'one expert': index == 3, 'all': torch.ones(T, k, dtype=torch.bool)}[drop]
+    slot = slot.masked_fill(gone.cuda(), -1)
+    named = torch.zeros(T * k, dtype=torch.bool, device='cuda')
+    named[slot[slot >= 0]] = True
+    acc = F64 if dtype == F64 else F32
+    few, many = rand(gen, T, K, dtype=dtype).cuda(), rand(gen, T * k, K, dtype=dtype).cuda()
+    weight = rand(gen, T, k, dtype=acc).cuda()
+    size = many.numel() * many.element_size()
+    rows_of = torch.zeros(T * k, dtype=torch.long, device='cuda')
+    rows_of[slot[slot >= 0]] = torch.arange(T, device='cuda').repeat_interleave(k).view(T, k)[slot >= 0]
+    for w in (None, weight):
+        leave_nan(size, size)
+        rows = ts.expert_dispatch(few, slot, indptr, w)
+        assert not bool(rows[~named].any())
+        if w is None:
+            assert torch.equal(rows[named], few[rows_of[named]])
+    for w, dots in ((None, False), (weight, False), (weight, True)):
+        leaf = many.clone().requires_grad_()
+        wl = None if w is None else w.clone().requires_grad_(dots)
+        out = ts.expert_combine(leaf, slot, indptr, wl)
+        leave_nan(size, size)
+        grads = torch.autograd.grad(out, [leaf] + ([wl] if dots else []), few)
+        assert not bool(grads[0][~named].any())
+        if w is None:
+            assert torch.equal(grads[0][named], few[rows_of[named]])
+        if dots:
+            assert bool((grads[1][slot < 0] == 0).all())
+
+
+@pytest.mark.parametrize('T,k,K', [(300, 4, 64), (4000, 4, 72), (4000, 4, 1024)])
+def test_dropped_entries_captured_and_on_two_streams(T, k, K):
+    """Plans with holes in a captured graph that is replayed with other slots, followed at once by a kernel that reads the
+    rows; two streams at a time."""
+    gen = torch.Generator().manual_seed(K)
+    x, w = rand(gen, T, K, dtype=BF16).cuda(), rand(gen, T, k).cuda()
+    many = rand(gen, T * k, K, dtype=BF16).cuda().requires_grad_()
+    plans = []
+    for i in range(3):
+        slot, _, p = ts.expert_sort(torch.randint(-i, 9, (T, k), generator=gen).cuda(), 9)
+        plans.append((slot.masked_fill(torch.rand(T, k, generator=gen).cuda() < 0.2 * i, -1), p))
+    at, ptr = plans[0][0].clone(), plans[0][1].clone()
+
+    def both(slot, p):
+        rows = ts.expert_dispatch(x, slot, p)
+        wl = w.detach().requires_grad_()
+        grads = torch.autograd.grad(ts.expert_combine(many, slot, p, wl), (many, wl), x)
+        return (rows + 1,) + tuple(g + 1 for g in grads)  # (a kernel that reads them at once)
+
+    def plain(slot, p):
+        named = slot >= 0
+        rows, grad = torch.zeros(T * k, K, dtype=BF16, device='cuda'), torch.zeros(T * k, K, dtype=BF16, device='cuda')
+        token = torch.arange(T, device='cuda').repeat_interleave(k).view(T, k)
+        rows[slot[named]] = x[token[named]]
+        grad[slot[named]] = (x[token[named]].float() * w[named].unsqueeze(1)).to(BF16)
+        return rows + 1, grad + 1
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both(at, ptr)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both(at, ptr)
+    for slot, p in plans + plans[::-1]:
+        at.copy_(slot)
+        ptr.copy_(p)
+        leave_nan(2 * T * k * K)
+        graph.replay()
+        for got, want in zip(out, plain(slot, p)):
+            assert torch.equal(got, want)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for stream, plan in zip(streams * 3, plans * 2):
+        with torch.cuda.stream(stream):
+            outs.append(both(*plan))
+    torch.cuda.synchronize()
+    for got, plan in zip(outs, plans * 2):
+        for a, b in zip(got, plain(*plan)):
+            assert torch.equal(a, b)
