@@ -3,6 +3,8 @@
 // ops_common.h).
 #include "ops_common.h"
 
+#include <ATen/MemoryOverlap.h>
+
 namespace tsb_ops {
 namespace {
 
@@ -178,6 +180,8 @@ torch::Tensor scan_step_impl(torch::Tensor src_, torch::Tensor gate_, torch::Ten
   auto out = torch::empty_like(src);
   const int64_t n = src.size(0), K = n > 0 ? src.numel() / n : 0, gates = n > 0 ? gate.numel() / n : 0;
   if (src.numel() == 0) return out;
+  for (const auto &t : {src, gate})  // (the state itself may be one of them: every value is read by the thread that replaces it)
+    TORCH_CHECK(at::get_overlap_status(state, t) != at::MemOverlapStatus::Partial, "scan_step: src and gate must not overlap the state in part");
   check_status(tsb_scan_step(src.data_ptr(), gate.data_ptr(), state.data_ptr(), out.data_ptr(), n, K, K / gates, state.stride(0), dtype_enum(src),
                              dtype_enum(gate), current_stream()),
                "tsb_scan_step");

@@ -17,7 +17,8 @@ def scan_csr(src: torch.Tensor, gate: torch.Tensor, indptr: torch.Tensor,
         gate: of ``src``'s shape, or 1 in trailing dimensions whose channels share a gate (``[T, heads, 1]`` against
             ``[T, heads, width]``); any other broadcast is expanded.  ``src``'s dtype, or float32 with 16-bit data.
             Products of gates over a few hundred rows have to be finite: meant for magnitudes up to 1.
-        indptr: ascending int64 offsets; leading dimensions broadcast against ``src``'s.
+        indptr: ascending int64 offsets, those beyond the rows ending at them; leading dimensions broadcast against
+            ``src``'s.
         state: optional start of each range, ``src``'s shape with one row for each range, float32 (float64 with
             float64 data).
 
@@ -43,7 +44,8 @@ def scan_step(src: torch.Tensor, gate: torch.Tensor, state: torch.Tensor) -> tor
         src: ``[n, ...]``, one row for each state.
         gate: as in :func:`scan_csr`.
         state: of ``src``'s shape, float32 (float64 with float64 data); each state contiguous, the states possibly apart
-            (a slice of a pool).  Must not require a gradient: this is the serving form.
+            (a slice of a pool).  Must not require a gradient: this is the serving form.  ``src`` and ``gate`` may be the
+            state itself, but not overlap it in part.
 
     Returns the new state rounded to ``src``'s dtype.
     """

@@ -295,3 +295,22 @@ def test_dropped_entries_captured_and_on_two_streams(T, k, K):
     for got, plan in zip(outs, plans * 2):
         for a, b in zip(got, plain(*plan)):
             assert torch.equal(a, b)
+
+
+def test_step_on_overlapping_memory():
+    """The state itself as src or gate is fine; other values of its memory would be read before or after they change."""
+    buf = torch.rand(24, device='cuda')
+    state, x, g = buf[:16].view(2, 8), torch.rand(2, 8, device='cuda'), torch.rand(2, 8, device='cuda')
+    for src, gate in ((buf[8:].view(2, 8), g), (x, buf[4:20].view(2, 8)), (x, buf[2:4].view(2, 1)), (buf[1:17].view(2, 8), g)):
+        before = buf.clone()
+        with pytest.raises(RuntimeError, match='overlap'):
+            ts.scan_step(src, gate, state)
+        assert torch.equal(buf, before)
+    u = ref.unit(F32)
+    for src, gate in ((state, g), (x, state)):
+        s64, g64, h64 = src.double().cpu(), gate.double().cpu(), state.double().cpu()
+        want = g64 * h64 + s64
+        out = ts.scan_step(src, gate, state)
+        tol = 2 * u * ((g64 * h64).abs() + s64.abs())
+        ref.assert_within(state, want, tol, 'state')
+        ref.assert_within(out, want, tol, 'out')
