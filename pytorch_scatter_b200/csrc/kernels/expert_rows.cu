@@ -602,10 +602,14 @@ template <typename T, bool SPREAD, bool ALIGNED, bool WRITE, bool ZERO> int laun
     return launch_status();
   };
   const auto with_j = [&](auto gn) {
-    if (p.k <= 2 || (SPREAD && !ALIGNED)) return go(std::integral_constant<int, 2>(), gn);
-    if constexpr (ALIGNED && WRITE)
-      if (p.k > 4) return go(std::integral_constant<int, 8>(), gn);
-    return go(std::integral_constant<int, 4>(), gn);
+    if constexpr (SPREAD && !ALIGNED) {
+      return go(std::integral_constant<int, 2>(), gn);
+    } else {
+      if (p.k <= 2) return go(std::integral_constant<int, 2>(), gn);
+      if constexpr (ALIGNED && WRITE)
+        if (p.k > 4) return go(std::integral_constant<int, 8>(), gn);
+      return go(std::integral_constant<int, 4>(), gn);
+    }
   };
   // Threads of a token: what its chunks keep busy, and a whole CTA where the tokens alone would not fill the GPU.
   const int64_t Kc = chunks_of<T, ALIGNED>(p.K);

@@ -511,8 +511,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
   char *s_src = smem + (RAGGED ? ty * (lx * SrcSlot::kBytes + 16) : tid * SrcSlot::kBytes);
   char *s_fwd = smem + kStages * R * kSrcRow + (RAGGED ? ty * (lx * FwdSlot::kBytes + 16) : tid * FwdSlot::kBytes);
   char *s_gate = smem + kStages * R * (kSrcRow + (BWD ? kFwdRow : 0)) + (RAGGED ? ty * (lx * GateSlot::kBytes + 16) : tid * GateSlot::kBytes);
-  int64_t tile = (int64_t)rank * L;                 // position of the CTA's tile
-  int64_t ahead = tile + ty * R;                    // position of the thread's next rows to load
+  int64_t ahead = (int64_t)rank * L + ty * R;       // position of the thread's next rows to load
   const int64_t at = b * p.E + row_of(ahead);
   const T *lsrc = src_lo + (have_src ? at * p.K + c0 : 0);
   const A *lfwd = fwd_lo + (BWD ? (at - 1) * p.K + c0 : 0);  // h of the row before
@@ -846,7 +845,6 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
     async_wait_all_but<kStages - 1>();
     if (RAGGED) __syncwarp();  // the chunks that the other lanes of a row copied are there
     tile_work(stage, par, set);
-    tile += step;
     os += tile_k;
     ow += tile_k;
     og += tile_gates;
