@@ -431,8 +431,9 @@ __global__ void __launch_bounds__(kThreads) rows_dot_kernel(RowsParams p) {
 // Folds, and spreads with dot products, of long aligned rows of many tokens.  Every warp runs a pipeline of its own: bulk
 // copies bring pieces of its tokens' rows into a ring in shared memory, two steps and more ahead of the step that is
 // worked on, so the bytes in flight depend neither on registers nor on occupancy.  Lane j carries the j-th choice.
-// (Combine of 32768 x 2 x 4096 bf16: 140 us against 170 with the rows in flight in registers; with the products, backward,
-// 234 against 256.  A plain spread has nothing to wait for but one load and stays with rows_kernel, 205 us against 225.)
+// (Combine of 32768 x 2 x 4096 bf16: 139 us against 170 with the rows in flight in registers; with the products, backward,
+// 234 against 256 without holes_kernel, 236 with it.  A plain spread has nothing to wait for but one load and stays with
+// rows_kernel, 205 us against 225, 209 with holes_kernel.)
 constexpr int kBulkWarps = 8, kBulkMostStages = 8, kBulkChunks = 2, kBulkMostDots = 8;
 constexpr int kBulkWarpBytes = 27 * 512;  // three steps of 9 pieces of 512 bytes; two CTAs fit an SM
 constexpr int kBulkSmem = kBulkWarps * kBulkWarpBytes;

@@ -7,7 +7,7 @@
 // the choice, not by HBM: of a few hundred logits, most are ruled out first.  The k-th largest of the 32 lane maxima is a
 // lower bound of the k-th largest logit; the logits that reach it, rarely more than 2 k, move to one register of the
 // warp, and the k rounds of the choice run on that register.  (65536 x 256 fp32, k = 8: 50 us, 87 with every round
-// over all registers; the backward, which writes, 25.)
+// over all registers; the backward, which writes, 25: it waits for its loads of weight, gradient and index.)
 #include "common.cuh"
 
 namespace tsb {

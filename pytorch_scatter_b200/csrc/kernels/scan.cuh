@@ -17,8 +17,8 @@
 // on by its CTAs' tiles, carrying the value along in registers, so that one launch covers any length without waiting on
 // anything but its own cluster.  The composition has a fixed shape: results do not vary from run to run.
 //
-// 65536 x 2048 bf16 in 37 segments: forward 176 us, 4.6 TB/s, with h kept in 32 bits for a backward 298 us, 4.5 TB/s,
-// backward 318 us, 5.1 TB/s; bound by the latency of a tile's chain of steps with eight warps on an SM.
+// 65536 x 2048 bf16 in 37 segments: forward 180 us, 4.5 TB/s, with h kept in 32 bits for a backward 299 us, 4.5 TB/s,
+// backward 323 us, 5.0 TB/s; bound by the latency of a tile's chain of steps with eight warps on an SM.
 //
 // A segment's first row (backward: its last) does not take the value from the row before: such a map is marked `reset`
 // and drops what comes in, so infinities and NaN of one segment never reach the next.  Tiles that no segment border
@@ -84,7 +84,7 @@ template <typename T, int VEC> struct Slot {
   }
 };
 
-// Rows that begin anywhere (60000 x 333 fp16 in 3001 segments, forward / backward: 126 / 204 us; one channel to a thread
+// Rows that begin anywhere (60000 x 333 fp16 in 3001 segments, forward / backward: 131 / 215 us; one channel to a thread
 // instead: 191 / 369, the latter with h in 16 bits): the lanes of a row share its aligned 16-byte chunks, n of them to a lane and one more, and a
 // lane shifts its values out of its own and the next one (the lanes of a row are lanes of one warp).
 template <typename X, int VEC> struct Ragged {
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kScanThreads + 32, ScanShape<T, G, VEC, SHARED
   using A = acc_t<T>;
   constexpr int R = S::kRows;
   // A ragged row is a few hundred instructions: unrolled, the loops over a thread's rows do not fit the instruction cache
-  // (60000 x 333 fp16 in 3001 segments: 243 us, most of it waiting for instructions, against 126).
+  // (60000 x 333 fp16 in 3001 segments: 243 us, most of it waiting for instructions, against 131).
   constexpr int kUnroll = RAGGED ? 1 : R;
 
 
@@ -917,7 +917,7 @@ template <typename T, typename G, int VEC, bool SHARED, bool BWD, bool RAGGED> i
   };
   // Work is spread over as many CTAs as the GPU holds.  Rows are cut into parts at segment borders where there are
   // segments enough (six to a part make parts of similar length), and over a cluster for the rest, since
-  // its CTAs wait for each other at every tile: 37 segments over 65536 x 2048 bf16 take 199 us with a cluster of 8 and
+  // its CTAs wait for each other at every tile: 37 segments over 65536 x 2048 bf16 took 199 us with a cluster of 8 and
   // one part, 174 with 2 and 4, 179 with 1 and 9.  Where that leaves half the GPU empty a tile gets fewer channels (down
   // to 32 bytes of a row) and more rows: one segment of 65536 x 1024 takes 139 us at 128 bytes of a row, 98 at 64 and 141
   // at 32, which no longer fit at once.
