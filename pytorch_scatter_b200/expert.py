@@ -26,7 +26,7 @@ def expert_topk(logits: torch.Tensor, k: int, normalize: bool = True) -> Tuple[t
     Returns ``(weight, index)``, both ``[..., k]``, float32 and int64, in descending order of the logits, ties towards
     the smaller index.  A logit of ``-inf`` is never chosen: where fewer than ``k`` others are left the index is -1 (an
     entry that :func:`expert_sort` drops) and the weight 0.  NaN ranks above everything and makes the token's weights
-    NaN.  ``weight`` is differentiable with respect to ``logits`` (once).
+    NaN.  ``weight`` is differentiable with respect to ``logits`` (once, in reverse mode).
     """
     return torch.ops.torch_scatter.expert_topk(logits, k, normalize)
 
@@ -56,7 +56,7 @@ def expert_dispatch(src: torch.Tensor, slot: torch.Tensor, indptr: torch.Tensor,
             by a slot of -1; two entries must not share a slot.
         weight: optional factors of ``slot``'s shape, float32 (float64 with float64 rows).
 
-    Returns ``[slot.numel(), ...]``; rows that no entry names, those behind ``indptr[-1]`` among them, are zero.  Differentiable (once) with respect to ``src``
+    Returns ``[slot.numel(), ...]``; rows that no entry names, those behind ``indptr[-1]`` among them, are zero.  Differentiable (once, in reverse mode) with respect to ``src``
     and ``weight``; bit-reproducible run to run.
     """
     return torch.ops.torch_scatter.expert_dispatch(src, slot, indptr, weight)
@@ -73,7 +73,7 @@ def expert_combine(rows: torch.Tensor, slot: torch.Tensor, indptr: torch.Tensor,
             by a slot of -1 (their rows get a gradient of zero); two entries must not share a slot.
         weight: optional factors of ``slot``'s shape, float32 (float64 with float64 rows).
 
-    Returns ``[*tokens, ...]``; tokens whose entries were all dropped are zero.  Differentiable (once) with respect to
+    Returns ``[*tokens, ...]``; tokens whose entries were all dropped are zero.  Differentiable (once, in reverse mode) with respect to
     ``rows`` and ``weight``; bit-reproducible run to run.
     """
     return torch.ops.torch_scatter.expert_combine(rows, slot, indptr, weight)

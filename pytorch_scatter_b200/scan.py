@@ -24,7 +24,7 @@ def scan_csr(src: torch.Tensor, gate: torch.Tensor, indptr: torch.Tensor,
 
     The recurrence runs in 32 bits (64 for float64) whatever the data's type and is rounded once per output.  Rows
     outside every range are 0 and get no gradient.  With 16-bit data a forward pass that will need the gates' gradient
-    keeps ``h`` in float32 as well.  Differentiable (once) with respect to ``src``, ``gate`` and
+    keeps ``h`` in float32 as well.  Differentiable (once, in reverse mode) with respect to ``src``, ``gate`` and
     ``state``; bit-reproducible run to run.
     """
     return torch.ops.torch_scatter.scan_csr(src, gate, indptr, state)

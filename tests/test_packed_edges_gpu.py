@@ -314,3 +314,57 @@ def test_step_on_overlapping_memory():
         tol = 2 * u * ((g64 * h64).abs() + s64.abs())
         ref.assert_within(state, want, tol, 'state')
         ref.assert_within(out, want, tol, 'out')
+
+
+def test_more_elements_than_32_bits_count():
+    """The last segment, and the last tokens, of arrays of more than 2^31 elements: the bits of the same rows by themselves."""
+    gen = torch.Generator(device='cuda').manual_seed(1)
+    E, tail = 66000, 500
+    for K in (33000, 32997):  # 2.18e9 elements, rows on a 16-byte boundary and off it
+        src = torch.rand(E, K, device='cuda', generator=gen, dtype=BF16)
+        gate = torch.rand(E, K, device='cuda', generator=gen, dtype=BF16)
+        p = torch.tensor([0, 3, E - tail, E], device='cuda')
+        out = ts.scan_csr(src.requires_grad_(), gate.requires_grad_(), p)
+        gs, gg = torch.autograd.grad(out, (src, gate), out.detach())
+        with torch.no_grad():
+            x, g = src[-tail:].clone().requires_grad_(), gate[-tail:].clone().requires_grad_()
+        # (cut into other tiles, so the roundings differ: both within a bf16 step of the exact values)
+        few = ts.scan_csr(x, g, torch.tensor([0, tail], device='cuda'))
+        fs, fg = torch.autograd.grad(few, (x, g), few.detach())
+        for a, b in ((out[-tail:], few), (gs[-tail:], fs), (gg[-tail:], fg)):
+            assert bool(((a.float() - b.float()).abs() <= 2.0 ** -6 * b.float().abs()).all())
+        del src, gate, out, gs, gg
+    T, k, K = 140000, 8, 2048  # 2.29e9 elements of rows
+    slot, order, ptr = ts.expert_sort(torch.randint(-1, 16, (T, k), device='cuda', generator=gen), 16)
+    x = torch.rand(T, K, device='cuda', generator=gen, dtype=BF16)
+    rows = ts.expert_dispatch(x, slot, ptr)
+    used = int(ptr[-1])
+    assert not bool(rows[used:].any())
+    for places in (slice(0, 1000), slice(used - 1000, used)):
+        assert torch.equal(rows[places], x[order[places] // k])
+    slot[-3:, :] = -1  # holes far behind
+    rows = ts.expert_dispatch(x, slot, ptr)
+    named = torch.zeros(T * k, dtype=torch.bool, device='cuda')
+    named[slot[slot >= 0]] = True
+    assert not bool(rows[~named].any())
+    w = torch.rand(T, k, device='cuda', generator=gen)
+    out = ts.expert_combine(rows, slot, ptr, w)
+    want = (rows[slot[-1003:-3].clamp_min(0)].double() * (w[-1003:-3] * (slot[-1003:-3] >= 0)).double().unsqueeze(-1)).sum(1)
+    assert bool(((out[-1003:-3].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-5 * want.abs()).all()) and not bool(out[-3:].any())
+
+
+def test_16_bit_recurrence_compiles():
+    """A traced training step keeps h in fp32 as the eager one does."""
+    gen = torch.Generator().manual_seed(3)
+    p = torch.tensor([0, 30, 31, 100], device='cuda')
+    x, g, s = rand(gen, 100, 24, dtype=BF16).cuda(), torch.sigmoid(rand(gen, 100, 24) + 1).to(BF16).cuda(), rand(gen, 3, 24).cuda()
+    d = rand(gen, 100, 24, dtype=BF16).cuda()
+
+    def step(f):
+        leaves = [t.clone().requires_grad_() for t in (x, g, s)]
+        out, last = f(*leaves)
+        return (out.detach(), last.detach()) + torch.autograd.grad((out, last), leaves, (d, torch.ones_like(last)))
+
+    f = lambda a, b, c: ts.scan_csr_state(a, b, p, c)  # noqa: E731
+    for got, want in zip(step(torch.compile(f, fullgraph=True)), step(f)):
+        assert torch.equal(got, want)
