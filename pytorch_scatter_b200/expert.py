@@ -56,8 +56,8 @@ def expert_dispatch(src: torch.Tensor, slot: torch.Tensor, indptr: torch.Tensor,
             by a slot of -1; two entries must not share a slot.
         weight: optional factors of ``slot``'s shape, float32 (float64 with float64 rows).
 
-    Returns ``[slot.numel(), ...]``; rows that no entry names, those behind ``indptr[-1]`` among them, are zero.  Differentiable (once, in reverse mode) with respect to ``src``
-    and ``weight``; bit-reproducible run to run.
+    Returns ``[slot.numel(), ...]``; rows that no entry names, those behind ``indptr[-1]`` among them, are zero.
+    Differentiable (once, in reverse mode) with respect to ``src`` and ``weight``; bit-reproducible run to run.
     """
     return torch.ops.torch_scatter.expert_dispatch(src, slot, indptr, weight)
 
@@ -73,7 +73,7 @@ def expert_combine(rows: torch.Tensor, slot: torch.Tensor, indptr: torch.Tensor,
             by a slot of -1 (their rows get a gradient of zero); two entries must not share a slot.
         weight: optional factors of ``slot``'s shape, float32 (float64 with float64 rows).
 
-    Returns ``[*tokens, ...]``; tokens whose entries were all dropped are zero.  Differentiable (once, in reverse mode) with respect to
-    ``rows`` and ``weight``; bit-reproducible run to run.
+    Returns ``[*tokens, ...]``; tokens whose entries were all dropped are zero.  Differentiable (once, in
+    reverse mode) with respect to ``rows`` and ``weight``; bit-reproducible run to run.
     """
     return torch.ops.torch_scatter.expert_combine(rows, slot, indptr, weight)
